@@ -206,6 +206,48 @@ GRAPH_SYMBOLS = {
     "butd_stream_destroy": (_c_int, [_P]),
 }
 
+
+class GatedFfnArgs(ctypes.Structure):
+    """ctypes mirror of ``butd_gated_ffn_args`` (include/butd_gated_ffn.h)."""
+    _fields_ = [("dtype", _c_int), ("activation", _c_int), ("rows", _c_long), ("width", _c_int), ("hidden", _c_int),
+                ("x", _P), ("w_gate", _P), ("w_up", _P), ("w_down", _P),
+                ("ld_x", _c_long), ("ld_gate", _c_long), ("ld_up", _c_long), ("ld_down", _c_long),
+                ("b_gate", _P), ("b_up", _P), ("b_down", _P),
+                ("h", _P), ("a", _P), ("b", _P), ("ld_h", _c_long), ("y", _P), ("ld_y", _c_long),
+                ("dy", _P), ("ld_dy", _c_long), ("dx", _P), ("ld_dx", _c_long),
+                ("dw_gate", _P), ("dw_up", _P), ("dw_down", _P), ("db_gate", _P), ("db_up", _P), ("db_down", _P)]
+
+
+GATED_FFN_SYMBOLS = {
+    "butd_gated_ffn_ld_hidden": (_c_long, [_c_int, _c_int]),
+    "butd_gated_ffn_set_tile": (_c_int, [_c_int, _c_int]),
+    "butd_gated_ffn_fwd_workspace": (_c_long, [ctypes.POINTER(GatedFfnArgs)]),
+    "butd_gated_ffn_bwd_workspace": (_c_long, [ctypes.POINTER(GatedFfnArgs)]),
+    "butd_gated_ffn_fwd": (_c_int, [ctypes.POINTER(GatedFfnArgs), _P, _c_long, _P]),
+    "butd_gated_ffn_bwd": (_c_int, [ctypes.POINTER(GatedFfnArgs), _P, _c_long, _P]),
+}
+
+
+class ResidualNormArgs(ctypes.Structure):
+    """ctypes mirror of ``butd_residual_norm_args`` (include/butd_residual_norm.h)."""
+    _fields_ = [("x_dtype", _c_int), ("stream_dtype", _c_int),
+                ("post_kind", _c_int), ("pre_kind", _c_int), ("gate_kind", _c_int),
+                ("post_dtype", _c_int), ("pre_dtype", _c_int), ("gate_dtype", _c_int),
+                ("rows", _c_long), ("rows_per_sample", _c_long), ("cols", _c_int),
+                ("residual_scale", _c_float), ("post_eps", _c_float), ("pre_eps", _c_float),
+                ("x", _P), ("residual", _P), ("gate", _P),
+                ("post_weight", _P), ("post_bias", _P), ("pre_weight", _P), ("pre_bias", _P),
+                ("stream", _P), ("normed", _P), ("stats", _P), ("d_stream", _P), ("d_normed", _P),
+                ("d_x", _P), ("d_residual", _P), ("d_gate", _P),
+                ("d_post_weight", _P), ("d_post_bias", _P), ("d_pre_weight", _P), ("d_pre_bias", _P)]
+
+
+RESIDUAL_NORM_SYMBOLS = {
+    "butd_residual_norm_fwd": (_c_int, [ctypes.POINTER(ResidualNormArgs), _P]),
+    "butd_residual_norm_bwd_workspace": (_c_long, [ctypes.POINTER(ResidualNormArgs)]),
+    "butd_residual_norm_bwd": (_c_int, [ctypes.POINTER(ResidualNormArgs), _P, _c_long, _P]),
+}
+
 ALL_SYMBOLS = dict(POINTNET2_SYMBOLS)
 ALL_SYMBOLS.update(ATTENTION_SYMBOLS)
 ALL_SYMBOLS.update(SA_SYMBOLS)
@@ -216,6 +258,8 @@ ALL_SYMBOLS.update(CRITERION_SYMBOLS)
 ALL_SYMBOLS.update(AUGMENT_SYMBOLS)
 ALL_SYMBOLS.update(GRAPH_SYMBOLS)
 ALL_SYMBOLS.update(ROWWISE_SYMBOLS)
+ALL_SYMBOLS.update(GATED_FFN_SYMBOLS)
+ALL_SYMBOLS.update(RESIDUAL_NORM_SYMBOLS)
 
 _lib = None
 

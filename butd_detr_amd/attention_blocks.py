@@ -139,3 +139,41 @@ def ffn_block(ffn, norm, x):
         from . import fused_attention
         return fused_attention.ffn_block(ffn, norm, x)
     return norm(x + ffn(x))
+
+
+def gated_ffn(ffn, x):
+    """W_down (act(W_gate x) * (W_up x)); ffn = gated_ffn.GatedFeedForward."""
+    if _BACKEND == "hip" and x.is_cuda:
+        from . import gated_ffn as fused
+        return fused.gated_ffn(x, ffn.gate.weight, ffn.up.weight, ffn.down.weight, ffn.gate.bias, ffn.up.bias,
+                               ffn.down.bias, activation=ffn.activation)
+    act = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda a: F.gelu(a, approximate="tanh"), "relu": F.relu,
+           "sigmoid": torch.sigmoid}[ffn.activation]
+    return ffn.down(act(ffn.gate(x)) * ffn.up(x))
+
+
+def residual_norm(x, residual=None, *, post_norm=None, gate=None, residual_scale=1.0, pre_norm=None):
+    """(stream, normed): stream = residual_scale * residual + gate * post_norm(x), normed = pre_norm(stream) | None."""
+    if _BACKEND == "hip" and x.is_cuda:
+        from . import residual_norm as fused
+        return fused.residual_norm(x, residual, post_norm=post_norm, gate=gate, residual_scale=residual_scale,
+                                   pre_norm=pre_norm)
+    branch = x if post_norm is None else post_norm(x)
+    if gate is not None:
+        branch = branch * (gate[:, None, :] if x.dim() == 3 and gate.dim() == 2 else gate)
+    stream = branch if residual is None else (residual_scale * residual + branch).to(residual.dtype)
+    return stream, None if pre_norm is None else pre_norm(stream).to(x.dtype)
+
+
+def gated_ffn_block(ffn, x, *, pre_norm=None, normed=None, post_norm=None, gate=None, residual_scale=1.0, next_norm=None):
+    """The pre-norm / sandwich-norm feed-forward block of a layer stack:
+        stream = residual_scale * x + gate * post_norm(FFN(pre_norm(x))),   FFN = gated_ffn(ffn, .)
+    -> (stream, next_norm(stream) | None).  ``next_norm``: the norm in front of the NEXT block, computed by the kernel that
+    writes the stream; that block then takes it as ``normed`` in place of ``pre_norm`` (a float32 stream around a 16-bit FFN
+    needs it: pre_norm alone would return the stream's type)."""
+    if (pre_norm is None) == (normed is None):
+        raise ValueError("gated_ffn_block: one of pre_norm and normed")
+    if normed is None:
+        normed = residual_norm(x, pre_norm=pre_norm)[1]
+    return residual_norm(gated_ffn(ffn, normed), x, post_norm=post_norm, gate=gate, residual_scale=residual_scale,
+                         pre_norm=next_norm)

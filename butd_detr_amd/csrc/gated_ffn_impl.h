@@ -1,0 +1,581 @@
+// gated_ffn_impl.h -- the gated feed-forward block for one tensor type T (include/butd_gated_ffn.h): the kernels around the
+// tile product (ffn_tile.h) and the host-side plan.  Instantiated by gated_ffn_f32 / _bf16 / _f16.hip.
+#pragma once
+#include "../../include/butd_gated_ffn.h"
+#include "ffn_tile.h"
+#include "zero_fill.h"
+
+namespace ffn {
+
+// ---- few rows -----------------------------------------------------------------------------------------------------------
+// Up to 64 rows: the product reads every weight once and little else, so it is a stream of weights with 16 rows (a matrix
+// instruction's width) per accumulator tile.  A workgroup owns 16 output columns; its waves share out the contraction in
+// 128-byte pieces (whole lines of the weights' rows), load straight into fragments -- nothing is reused between waves, LDS
+// would only add a trip -- and join their sums in LDS.
+template <typename T, bool AL> __device__ inline u32x4 load_unit(const T *p, int left) {
+  u32x4 v;
+  if constexpr (AL) {
+    v = left > 0 ? *(const u32x4 *)p : u32x4{0, 0, 0, 0};
+  } else {
+    if (left >= Num<T>::kVec) {
+      __builtin_memcpy(&v, p, 16);                       // rows at odd addresses: unaligned vector loads
+    } else {
+      T e[Num<T>::kVec];
+#pragma unroll
+      for (int i = 0; i < Num<T>::kVec; ++i) e[i] = i < left ? p[i] : (T)0.f;
+      __builtin_memcpy(&v, e, 16);
+    }
+  }
+  return v;
+}
+
+struct FewRows {
+  const void *x, *w0, *w1;     // ld in elements
+  long ldx, ldw0, ldw1;
+  int M, N, K, act;
+  void *c;
+  long ldc;
+  int pad;
+  const void *bias0, *bias1;
+  float *out0, *out1;
+  long ldaux;
+};
+
+template <typename T, int PARTS, int MT, bool AL, int NW>
+__global__ __launch_bounds__(NW * 64) void few_rows_kernel(const FewRows P) {
+  constexpr int kVec = Num<T>::kVec, kStep = 8 * kVec;   // 128 bytes of a row
+  __shared__ f32x4 part[NW][PARTS * MT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int nrow = min(n0 + i, P.N - 1);                 // rows behind the last repeat it; their results are not stored
+  const T *w[PARTS];
+  w[0] = (const T *)P.w0 + (long)nrow * P.ldw0 + g * kVec;
+  if constexpr (PARTS == 2) w[1] = (const T *)P.w1 + (long)nrow * P.ldw1 + g * kVec;
+  const T *x[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) x[t] = (const T *)P.x + (long)min(16 * t + i, P.M - 1) * P.ldx + g * kVec;
+  f32x4 acc[PARTS][MT];
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[p][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // kAhead pieces' loads are issued before the first of them is used (units past the contraction's end arrive as zeros)
+  constexpr int kAhead = MT == 4 ? 2 : 4;
+  for (int k = wave * kStep; k < P.K; k += kAhead * NW * kStep) {
+    u32x4 fw[kAhead][2][PARTS], fx[kAhead][2][MT];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int kk = k + u * NW * kStep + s * 4 * kVec, left = P.K - kk - g * kVec;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) fw[u][s][p] = load_unit<T, AL>(w[p] + kk, left);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) fx[u][s][t] = load_unit<T, AL>(x[t] + kk, left);
+      }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+          for (int t = 0; t < MT; ++t) acc[p][t] = mma(fw[u][s][p], fx[u][s][t], acc[p][t], (const T *)nullptr);
+  }
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) part[wave][p * MT + t][lane] = acc[p][t];
+  __syncthreads();
+  if (wave >= MT) return;
+  const int t = wave, m = 16 * t + i, n = n0 + 4 * g;
+  f32x4 sum[PARTS];
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    sum[p] = part[0][p * MT + t][lane];
+    for (int v = 1; v < NW; ++v) sum[p] += part[v][p * MT + t][lane];
+  }
+  if (m >= P.M) return;
+  float v[PARTS][4];
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const void *bias = p ? P.bias1 : P.bias0;
+      v[p][e] = sum[p][e] + (bias && n + e < P.N ? (float)((const T *)bias)[n + e] : 0.f);
+    }
+  T *row = (T *)P.c + (long)m * P.ldc;
+  const bool whole = (P.ldc & 3) == 0 && ((uintptr_t)P.c & 15) == 0;
+  if constexpr (PARTS == 2) {
+    float h[4], slope[4];
+    activation4(P.act, v[0], h, slope);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] *= v[1][e];
+    put<T>(row, n, P.N, P.pad, whole, h);
+    if (P.out0) {
+      put<float>(P.out0 + (long)m * P.ldaux, n, P.N, 0, true, v[0]);
+      put<float>(P.out1 + (long)m * P.ldaux, n, P.N, 0, true, v[1]);
+    }
+  } else {
+    put<T>(row, n, P.N, 0, whole, v[0]);
+  }
+}
+
+// ---- rows that direct loads cannot take -----------------------------------------------------------------------------------
+struct Copy {
+  const void *src;
+  void *dst;
+  long rows, ld_src, ld_dst;   // elements
+  int cols;
+  long first;                  // first block
+};
+constexpr int kMaxCopies = 5;
+struct Copies {
+  Copy c[kMaxCopies];
+  int count;
+};
+// 16-byte units of the destination, zeros behind the last column
+template <typename T> __global__ __launch_bounds__(256) void copy_rows_kernel(const Copies L) {
+  int ci = 0;
+#pragma unroll
+  for (int i = 1; i < kMaxCopies; ++i)
+    if (i < L.count && (long)blockIdx.x >= L.c[i].first) ci = i;
+  const Copy C = L.c[ci];
+  const long unit = ((long)blockIdx.x - C.first) * 256 + threadIdx.x;
+  const int per_row = (int)(C.ld_dst / Num<T>::kVec);
+  const long row = unit / per_row;
+  if (row >= C.rows) return;
+  const int col = (int)(unit - row * per_row) * Num<T>::kVec;
+  *(u32x4 *)((T *)C.dst + row * C.ld_dst + col) = load_unit<T, false>((const T *)C.src + row * C.ld_src + col, C.cols - col);
+}
+
+// ---- slabs of a split contraction -----------------------------------------------------------------------------------------
+struct Fold {
+  const float *slab;
+  long stride;
+  int split, M, N;
+  void *c;
+  long ldc;
+  const void *bias;
+  long first;
+};
+struct Folds {
+  Fold f[kMaxProblems];
+  int count;
+};
+template <typename T> __global__ __launch_bounds__(256) void fold_kernel(const Folds L) {
+  int fi = 0;
+#pragma unroll
+  for (int i = 1; i < kMaxProblems; ++i)
+    if (i < L.count && (long)blockIdx.x >= L.f[i].first) fi = i;
+  const Fold F = L.f[fi];
+  const long quads = (F.N + 3) / 4, q = ((long)blockIdx.x - F.first) * 256 + threadIdx.x;
+  const long m = q / quads;
+  if (m >= F.M) return;
+  const int n = (int)(q - m * quads) * 4;
+  const float *src = F.slab + m * F.N + n;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if ((F.N & 3) == 0) {
+    f32x4 s = *(const f32x4 *)src;
+    for (int i = 1; i < F.split; ++i) s += *(const f32x4 *)(src + i * F.stride);      // in slice order: reproducible
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = s[e];
+  } else {
+    for (int i = 0; i < F.split; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < F.N) v[e] += src[i * F.stride + e];
+  }
+  if (F.bias) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < F.N) v[e] += (float)((const T *)F.bias)[n + e];
+  }
+  put<T>((T *)F.c + m * F.ldc, n, F.N, 0, (F.ldc & 3) == 0 && ((uintptr_t)F.c & 15) == 0, v);
+}
+
+// ---- bias gradients -------------------------------------------------------------------------------------------------------
+struct ColumnSum {
+  const void *src;
+  long ld;                     // elements
+  int cols;
+  float *part;                 // (chunks, cols)
+  void *out;
+  int first;                   // first column block
+};
+struct ColumnSums {
+  ColumnSum c[3];
+  int count, chunks;
+  long rows;
+};
+template <typename T> __global__ __launch_bounds__(256) void column_sum_kernel(const ColumnSums L) {
+  int ci = 0;
+#pragma unroll
+  for (int i = 1; i < 3; ++i)
+    if (i < L.count && (int)blockIdx.x >= L.c[i].first) ci = i;
+  const ColumnSum C = L.c[ci];
+  const int col = ((int)blockIdx.x - C.first) * 64 + (threadIdx.x & 63), sub = threadIdx.x >> 6;
+  const long per = (L.rows + L.chunks - 1) / L.chunks, r0 = blockIdx.y * per, r1 = min(L.rows, r0 + per);
+  float s = 0.f;
+  if (col < C.cols) {
+    const T *p = (const T *)C.src + col;
+#pragma unroll 8
+    for (long r = r0 + sub; r < r1; r += 4) s += (float)p[r * C.ld];
+  }
+  __shared__ float sums[4][64];
+  sums[sub][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (sub == 0 && col < C.cols)
+    C.part[(long)blockIdx.y * C.cols + col] = (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
+}
+template <typename T> __global__ __launch_bounds__(256) void column_sum_fold_kernel(const ColumnSums L) {
+  int ci = 0;
+#pragma unroll
+  for (int i = 1; i < 3; ++i)
+    if (i < L.count && (int)blockIdx.x >= L.c[i].first) ci = i;
+  const ColumnSum C = L.c[ci];
+  const int lane = threadIdx.x & 63, sub = threadIdx.x >> 6;
+  const int col = ((int)blockIdx.x - C.first) * 64 + lane;
+  float s = 0.f;
+  if (col < C.cols)
+    for (int k = sub; k < L.chunks; k += 4) s += C.part[(long)k * C.cols + col];
+  __shared__ float sums[4][64];
+  sums[sub][lane] = s;
+  __syncthreads();
+  if (sub == 0 && col < C.cols) ((T *)C.out)[col] = (T)((sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]));
+}
+
+// ---- plan -----------------------------------------------------------------------------------------------------------------
+constexpr int kCUs = 256;
+constexpr long kMaxLd = 1L << 22;      // bytes between rows: 256 rows of a tile stay within a buffer descriptor's 2 GB
+
+struct Arena {                         // carves the workspace; with a null base it only counts
+  char *base;
+  long used = 0;
+  void *take(long bytes) {
+    char *p = base ? base + used : nullptr;
+    used += (bytes + 255) / 256 * 256;
+    return p;
+  }
+};
+
+enum Layout { kNT, kNN, kTN };         // A and B K-contiguous; B K-strided; both K-strided
+
+struct TileChoice {
+  int size, split;                     // 256, 128 or 64
+};
+
+// butd_gated_ffn_set_tile: (0, 0) = the rule below
+extern int forced_tile, forced_split;
+
+// Which tile, and into how many slices the contraction is cut (products whose slabs can be folded only).  Modelled time: the
+// tiles of a launch go round the chip in ceil(tiles / 256) turns (one tile per CU and turn), each turn costs the tile's
+// multiplications at the rate measured for that tile; slabs are written and read once at about 4 TB/s plus one launch.
+struct Shape {
+  long M, N;
+};
+template <typename T> inline TileChoice choose(const Shape *shapes, int count, long k, bool can_split) {
+  // multiply-adds per CU and microsecond at full occupancy, large sizes (see the table at the launches)
+  static const double rate16[3] = {2.2e6, 1.6e6, 0.8e6}, rate32[3] = {0, 0.22e6, 0.17e6};
+  const double *rate = sizeof(T) == 2 ? rate16 : rate32;
+  static const int sizes[3] = {256, 128, 64};
+  if (forced_tile) return TileChoice{sizeof(T) == 4 && forced_tile == 256 ? 128 : forced_tile, can_split ? forced_split : 1};
+  TileChoice best{64, 1};
+  double best_us = 1e30;
+  for (int c = 0; c < 3; ++c) {
+    if (rate[c] == 0) continue;
+    const int t = sizes[c];
+    double tiles = 0, elems = 0;
+    for (int i = 0; i < count; ++i) {
+      tiles += (double)((shapes[i].M + t - 1) / t) * (double)((shapes[i].N + t - 1) / t);
+      elems += (double)shapes[i].M * (double)shapes[i].N;
+    }
+    for (int s = 1; s <= 64; s *= 2) {
+      if (s > 1 && (!can_split || k / s < 4 * Num<T>::kBK)) break;
+      const double turns = (double)(long)((tiles * s + kCUs - 1) / kCUs);
+      double us = turns * t * t * ((double)k / s + 2 * Num<T>::kBK) / rate[c];
+      if (s > 1) us += 3.0 + elems * 4 * (s + 1) / 4e6;
+      if (us < best_us) {
+        best_us = us;
+        best = TileChoice{t, s};
+      }
+    }
+  }
+  return best;
+}
+
+template <class C> inline hipError_t launch_tiles(Launch &L, hipStream_t stream) {
+  long total = 0;
+  constexpr int nw = C::kind == kGateUp ? C::TN / 2 : C::TN;
+  for (int i = 0; i < L.count; ++i) {
+    Problem &p = L.p[i];
+    const long tm = ((long)p.M + C::TM - 1) / C::TM, tn = ((long)p.N + nw - 1) / nw;
+    if (tm * tn * p.split > 0x7fffffffL - total) return hipErrorInvalidValue;
+    p.tiles_m = (int)tm;
+    p.tiles_n = (int)tn;
+    p.first = (int)total;
+    total += tm * tn * p.split;
+  }
+  L.total = (int)total;
+  hipLaunchKernelGGL((tile_kernel<C>), dim3((unsigned)total), dim3(C::kThreads), 0, stream, L);
+  return hipGetLastError();
+}
+
+// The tile kernels of one type.  (Named here: from the launches alone hipcc leaves the host side of some of them out.)
+#define BUTD_FFN_TILES(T, TM, WM, WN, WM1, WN1)                                                \
+  template __global__ void tile_kernel<Config<T, kGateUp, true, true, TM, TM, WM1, WN1>>(const Launch); \
+  template __global__ void tile_kernel<Config<T, kPlain, true, true, TM, TM, WM, WN>>(const Launch);   \
+  template __global__ void tile_kernel<Config<T, kPlain, true, false, TM, TM, WM, WN>>(const Launch);  \
+  template __global__ void tile_kernel<Config<T, kPlain, false, false, TM, TM, WM, WN>>(const Launch); \
+  template __global__ void tile_kernel<Config<T, kGrad, true, false, TM, TM, WM, WN>>(const Launch);
+
+// The three tiles of every kind.  The smallest of kGateUp has its waves stacked along m: a wave holds both parts of its columns.
+template <typename T, int KIND, Layout LAY> inline hipError_t run_tiles(Launch &L, int size, hipStream_t stream) {
+  constexpr bool ak = LAY != kTN, bk = LAY == kNT;
+  if constexpr (sizeof(T) == 2) {
+    if (size == 256) return launch_tiles<Config<T, KIND, ak, bk, 256, 256, 2, 4>>(L, stream);
+  }
+  if (size == 128) return launch_tiles<Config<T, KIND, ak, bk, 128, 128, 2, 2>>(L, stream);
+  if constexpr (KIND == kGateUp) return launch_tiles<Config<T, KIND, ak, bk, 64, 64, 4, 1>>(L, stream);
+  else return launch_tiles<Config<T, KIND, ak, bk, 64, 64, 2, 2>>(L, stream);
+}
+
+template <typename T> struct Block {
+  static constexpr int kVec = Num<T>::kVec;
+  static constexpr long kFewRows = 64;
+
+  // an operand as the tile product takes it: itself, or a copy with aligned rows in the workspace
+  struct Operand {
+    const void *p;
+    long ld;                                             // elements
+  };
+  struct Packer {
+    Arena &ws;
+    Copies L;
+    long blocks = 0;
+    explicit Packer(Arena &a) : ws(a) { L.count = 0; }
+    static bool direct(const void *p, long ld, int cols) {
+      return ((uintptr_t)p & 15) == 0 && ld % kVec == 0 && cols % kVec == 0 && ld * (long)sizeof(T) <= kMaxLd;
+    }
+    Operand pack(const void *p, long ld, long rows, int cols) {
+      const long ld_dst = (cols + kVec - 1) / kVec * kVec;
+      void *dst = ws.take(rows * ld_dst * (long)sizeof(T));
+      L.c[L.count++] = Copy{p, dst, rows, ld, ld_dst, cols, blocks};
+      blocks += (rows * (ld_dst / kVec) + 255) / 256;
+      return Operand{dst, ld_dst};
+    }
+    Operand take(const void *p, long ld, long rows, int cols) {
+      return direct(p, ld, cols) ? Operand{p, ld} : pack(p, ld, rows, cols);
+    }
+    hipError_t run(hipStream_t stream) {
+      if (!L.count) return hipSuccess;
+      if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
+      hipLaunchKernelGGL((copy_rows_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, L);
+      return hipGetLastError();
+    }
+  };
+  // the two projections share one row stride in the product
+  static void take_pair(Packer &pk, const butd_gated_ffn_args &A, Operand &gate, Operand &up) {
+    if (A.ld_gate == A.ld_up && Packer::direct(A.w_gate, A.ld_gate, A.width) && Packer::direct(A.w_up, A.ld_up, A.width)) {
+      gate = Operand{A.w_gate, A.ld_gate};
+      up = Operand{A.w_up, A.ld_up};
+    } else {
+      gate = pk.pack(A.w_gate, A.ld_gate, A.hidden, A.width);
+      up = pk.pack(A.w_up, A.ld_up, A.hidden, A.width);
+    }
+  }
+  static void operands(Problem &p, Operand a, Operand b) {
+    p.a[0] = p.a[1] = a.p;
+    p.b[0] = p.b[1] = b.p;
+    p.lda = a.ld * (long)sizeof(T);
+    p.ldb = b.ld * (long)sizeof(T);
+    p.segments = 1;
+    p.split = 1;
+  }
+  static hipError_t fold(const Launch &L, hipStream_t stream) {
+    Folds F;
+    F.count = 0;
+    long blocks = 0;
+    for (int i = 0; i < L.count; ++i) {
+      const Problem &p = L.p[i];
+      if (p.split == 1) continue;
+      F.f[F.count++] = Fold{p.slab, p.slab_stride, p.split, p.M, p.N, p.c, p.ldc, p.bias0, blocks};
+      blocks += ((long)p.M * ((p.N + 3) / 4) + 255) / 256;
+    }
+    if (!F.count) return hipSuccess;
+    if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((fold_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, F);
+    return hipGetLastError();
+  }
+  static void slabs(Launch &L, int split, Arena &ws) {
+    for (int i = 0; i < L.count; ++i) {
+      Problem &p = L.p[i];
+      const int steps = (p.K + Num<T>::kBK - 1) / Num<T>::kBK * p.segments;
+      const int per = (steps + split - 1) / split;
+      p.split = (steps + per - 1) / per;                 // every slice owns at least one step
+      if (p.split > 1) {
+        p.slab_stride = ((long)p.M * p.N + 3) / 4 * 4;
+        p.slab = (float *)ws.take(p.slab_stride * p.split * 4);
+      }
+    }
+  }
+
+  template <int PARTS> static hipError_t few_rows(const FewRows &P, hipStream_t stream) {
+    const bool al = (((uintptr_t)P.x | (uintptr_t)P.w0 | (uintptr_t)P.w1) & 15) == 0 && P.ldx % kVec == 0 && P.ldw0 % kVec == 0 &&
+                    P.ldw1 % kVec == 0 && P.K % kVec == 0;
+    const dim3 grid((unsigned)((P.N + 15) / 16));
+#define BUTD_FEW_ROWS(MT, AL) hipLaunchKernelGGL((few_rows_kernel<T, PARTS, MT, AL, 8>), grid, dim3(512), 0, stream, P)
+    if (P.M <= 16) {
+      if (al) BUTD_FEW_ROWS(1, true); else BUTD_FEW_ROWS(1, false);
+    } else if (P.M <= 32) {
+      if (al) BUTD_FEW_ROWS(2, true); else BUTD_FEW_ROWS(2, false);
+    } else {
+      if (al) BUTD_FEW_ROWS(4, true); else BUTD_FEW_ROWS(4, false);
+    }
+#undef BUTD_FEW_ROWS
+    return hipGetLastError();
+  }
+
+  // run == false: only count the workspace
+  static hipError_t forward(const butd_gated_ffn_args &A, Arena &ws, bool run, hipStream_t stream) {
+    const int M = (int)A.rows, E = A.width, F = A.hidden;
+    if (M == 0) return hipSuccess;
+    hipError_t err;
+    if (M <= kFewRows) {
+      if (!run) return hipSuccess;
+      FewRows P{A.x, A.w_gate, A.w_up, A.ld_x, A.ld_gate, A.ld_up, M, F, E, A.activation, A.h, A.ld_h, (int)A.ld_h,
+                A.b_gate, A.b_up, A.a, A.b, A.ld_h};
+      if ((err = few_rows<2>(P, stream)) != hipSuccess) return err;
+      FewRows D{A.h, A.w_down, A.w_down, A.ld_h, A.ld_down, A.ld_down, M, E, F, A.activation, A.y, A.ld_y, 0,
+                A.b_down, nullptr, nullptr, nullptr, 0};
+      return few_rows<1>(D, stream);
+    }
+    Packer pk(ws);
+    Operand x = pk.take(A.x, A.ld_x, M, E), gate, up;
+    take_pair(pk, A, gate, up);
+    Operand down = pk.take(A.w_down, A.ld_down, E, F);
+    Launch G{}, D{};
+    G.count = D.count = 1;
+    G.act = D.act = A.activation;
+    Problem &g = G.p[0], &d = D.p[0];
+    operands(g, x, gate);
+    g.b[1] = up.p;
+    g.M = M; g.N = F; g.K = E;
+    g.c = A.h; g.ldc = A.ld_h; g.pad = (int)A.ld_h;
+    g.bias0 = A.b_gate; g.bias1 = A.b_up;
+    g.out0 = A.a; g.out1 = A.b; g.ldaux = A.ld_h;
+    operands(d, Operand{A.h, A.ld_h}, down);
+    d.M = M; d.N = E; d.K = F;
+    d.c = A.y; d.ldc = A.ld_y; d.bias0 = A.b_down;
+    const Shape gs{M, 2L * F}, ds{M, E};
+    const TileChoice gc = choose<T>(&gs, 1, E, false), dc = choose<T>(&ds, 1, F, true);
+    slabs(D, dc.split, ws);
+    if (!run) return hipSuccess;
+    if ((err = pk.run(stream)) != hipSuccess) return err;
+    if ((err = run_tiles<T, kGateUp, kNT>(G, gc.size, stream)) != hipSuccess) return err;
+    if ((err = run_tiles<T, kPlain, kNT>(D, dc.size, stream)) != hipSuccess) return err;
+    return fold(D, stream);
+  }
+
+  static hipError_t backward(const butd_gated_ffn_args &A, Arena &ws, bool run, hipStream_t stream) {
+    const int M = (int)A.rows, E = A.width, F = A.hidden;
+    hipError_t err;
+    const bool inner = A.dx || A.dw_gate || A.dw_up || A.db_gate || A.db_up;    // da, db wanted
+    if (M == 0) {                                        // sums over nothing
+      if (!run) return hipSuccess;
+      void *const w[3] = {A.dw_gate, A.dw_up, A.dw_down}, *const b[3] = {A.db_gate, A.db_up, A.db_down};
+      for (int i = 0; i < 3; ++i) {
+        if (w[i] && (err = butd_zero_async(w[i], (size_t)E * F * sizeof(T), stream)) != hipSuccess) return err;
+        if (b[i] && (err = butd_zero_async(b[i], (size_t)(i == 2 ? E : F) * sizeof(T), stream)) != hipSuccess) return err;
+      }
+      return hipSuccess;
+    }
+    Packer pk(ws);
+    Operand x{}, gate{}, up{}, down{}, dy{};
+    if (inner || A.dw_down) dy = pk.take(A.dy, A.ld_dy, M, E);
+    if (A.dw_gate || A.dw_up) x = pk.take(A.x, A.ld_x, M, E);
+    if (A.dx) take_pair(pk, A, gate, up);
+    Operand da{}, db{};
+    Launch G{}, X{}, W{};
+    TileChoice gc{64, 1}, xc{64, 1}, wc{64, 1};
+    if (inner) {
+      down = pk.take(A.w_down, A.ld_down, E, F);
+      da = Operand{ws.take(A.ld_h * (long)M * (long)sizeof(T)), A.ld_h};
+      db = Operand{ws.take(A.ld_h * (long)M * (long)sizeof(T)), A.ld_h};
+      G.count = 1;
+      G.act = A.activation;
+      Problem &g = G.p[0];
+      operands(g, dy, down);
+      g.M = M; g.N = F; g.K = E;
+      g.c = (void *)da.p; g.c2 = (void *)db.p; g.ldc = A.ld_h; g.pad = (int)A.ld_h;
+      g.aux0 = A.a; g.aux1 = A.b; g.ldaux = A.ld_h;
+      const Shape s{M, F};
+      gc = choose<T>(&s, 1, E, false);
+    }
+    if (A.dx) {
+      X.count = 1;
+      Problem &p = X.p[0];
+      operands(p, da, gate);
+      p.a[1] = db.p; p.b[1] = up.p;
+      p.segments = 2;
+      p.M = M; p.N = E; p.K = F;
+      p.c = A.dx; p.ldc = A.ld_dx;
+      const Shape s{M, E};
+      xc = choose<T>(&s, 1, 2L * F, true);
+      slabs(X, xc.split, ws);
+    }
+    Shape ws_shapes[3];
+    auto weight = [&](Operand a, Operand b, int m, int n, void *c) {
+      ws_shapes[W.count] = Shape{m, n};
+      Problem &p = W.p[W.count++];
+      operands(p, a, b);
+      p.M = m; p.N = n; p.K = M;
+      p.c = c; p.ldc = n;
+    };
+    if (A.dw_gate) weight(da, x, F, E, A.dw_gate);
+    if (A.dw_up) weight(db, x, F, E, A.dw_up);
+    if (A.dw_down) weight(dy, Operand{A.h, A.ld_h}, E, F, A.dw_down);
+    if (W.count) {
+      wc = choose<T>(ws_shapes, W.count, M, true);
+      slabs(W, wc.split, ws);
+    }
+    // bias gradients: column sums of da, db, dy in row chunks
+    ColumnSums S;
+    S.count = 0;
+    S.rows = M;
+    int blocks = 0;
+    auto column = [&](const void *src, long ld, int cols, void *out) {
+      S.c[S.count++] = ColumnSum{src, ld, cols, nullptr, out, blocks};
+      blocks += (cols + 63) / 64;
+    };
+    if (A.db_gate) column(da.p, A.ld_h, F, A.db_gate);
+    if (A.db_up) column(db.p, A.ld_h, F, A.db_up);
+    if (A.db_down) column(A.dy, A.ld_dy, E, A.db_down);
+    if (S.count) {
+      long chunks = (8L * kCUs + blocks - 1) / blocks;   // about eight workgroups per CU, at least 32 rows each
+      const long most = ((long)M + 31) / 32;
+      S.chunks = (int)(chunks < 1 ? 1 : (chunks > most ? most : chunks));
+      for (int i = 0; i < S.count; ++i) S.c[i].part = (float *)ws.take((long)S.chunks * S.c[i].cols * 4);
+    }
+    if (!run) return hipSuccess;
+    if ((err = pk.run(stream)) != hipSuccess) return err;
+    if (inner && (err = run_tiles<T, kGrad, kNN>(G, gc.size, stream)) != hipSuccess) return err;
+    if (S.count) {
+      hipLaunchKernelGGL((column_sum_kernel<T>), dim3((unsigned)blocks, (unsigned)S.chunks), dim3(256), 0, stream, S);
+      if ((err = hipGetLastError()) != hipSuccess) return err;
+      hipLaunchKernelGGL((column_sum_fold_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, S);
+      if ((err = hipGetLastError()) != hipSuccess) return err;
+    }
+    if (A.dx) {
+      if ((err = run_tiles<T, kPlain, kNN>(X, xc.size, stream)) != hipSuccess) return err;
+      if ((err = fold(X, stream)) != hipSuccess) return err;
+    }
+    if (W.count) {
+      if ((err = run_tiles<T, kPlain, kTN>(W, wc.size, stream)) != hipSuccess) return err;
+      if ((err = fold(W, stream)) != hipSuccess) return err;
+    }
+    return hipSuccess;
+  }
+};
+
+}  // namespace ffn

@@ -1,0 +1,88 @@
+// gated_ffn_ops.hip -- entry points of include/butd_gated_ffn.h: checks of the arguments, dispatch on the tensors' type.
+#include "gated_ffn_impl.h"
+
+#define BUTD_FFN_DECLARE(T)                                                                            \
+  hipError_t butd_ffn_forward_##T(const butd_gated_ffn_args &, ffn::Arena &, bool, hipStream_t);       \
+  hipError_t butd_ffn_backward_##T(const butd_gated_ffn_args &, ffn::Arena &, bool, hipStream_t);
+BUTD_FFN_DECLARE(f32)
+BUTD_FFN_DECLARE(bf16)
+BUTD_FFN_DECLARE(f16)
+
+namespace ffn {
+int forced_tile = 0, forced_split = 0;
+}
+
+namespace {
+
+bool valid(const butd_gated_ffn_args *a, bool backward) {
+  if (!a || a->dtype < BUTD_FFN_F32 || a->dtype > BUTD_FFN_F16) return false;
+  if (a->activation < BUTD_FFN_SILU || a->activation > BUTD_FFN_SIGMOID) return false;
+  if (a->rows < 0 || a->rows > 0x7fffffffL || a->width < 1 || a->hidden < 1) return false;
+  // (a tile's last column index, and twice the hidden width, have to fit an int)
+  if (a->width > (1 << 28) || a->hidden > (1 << 28)) return false;
+  if (a->ld_gate < a->width || a->ld_up < a->width || a->ld_down < a->hidden) return false;
+  if (a->ld_h != butd_gated_ffn_ld_hidden(a->dtype, a->hidden)) return false;
+  if (a->rows == 0) return true;
+  const uintptr_t size = a->dtype == BUTD_FFN_F32 ? 4 : 2;
+  const void *const elements[] = {a->x, a->w_gate, a->w_up, a->w_down, a->b_gate, a->b_up, a->b_down, a->y, a->dy, a->dx,
+                                  a->dw_gate, a->dw_up, a->dw_down, a->db_gate, a->db_up, a->db_down};
+  for (const void *p : elements)
+    if ((uintptr_t)p % size) return false;
+  if (!a->x || a->ld_x < a->width || !a->w_gate || !a->w_up || !a->w_down) return false;
+  if (!a->h || ((uintptr_t)a->h | (uintptr_t)a->a | (uintptr_t)a->b) & 15) return false;
+  if ((a->a == nullptr) != (a->b == nullptr)) return false;
+  if (!backward) return a->y && a->ld_y >= a->width;
+  return a->a && a->dy && a->ld_dy >= a->width && (!a->dx || a->ld_dx >= a->width);
+}
+
+hipError_t dispatch(const butd_gated_ffn_args &a, ffn::Arena &ws, bool run, hipStream_t stream, bool backward) {
+  switch (a.dtype) {
+    case BUTD_FFN_F32: return backward ? butd_ffn_backward_f32(a, ws, run, stream) : butd_ffn_forward_f32(a, ws, run, stream);
+    case BUTD_FFN_BF16: return backward ? butd_ffn_backward_bf16(a, ws, run, stream) : butd_ffn_forward_bf16(a, ws, run, stream);
+    default: return backward ? butd_ffn_backward_f16(a, ws, run, stream) : butd_ffn_forward_f16(a, ws, run, stream);
+  }
+}
+
+long workspace(const butd_gated_ffn_args *a, bool backward) {
+  if (!valid(a, backward)) return -(long)hipErrorInvalidValue;
+  ffn::Arena ws{nullptr};
+  const hipError_t err = dispatch(*a, ws, false, nullptr, backward);
+  return err == hipSuccess ? ws.used : -(long)err;
+}
+
+int execute(const butd_gated_ffn_args *a, void *ws_ptr, long ws_bytes, butd_stream_t stream, bool backward) {
+  const long need = workspace(a, backward);
+  if (need < 0) return (int)-need;
+  if (need > 0 && (!ws_ptr || ws_bytes < need || ((uintptr_t)ws_ptr & 15))) return (int)hipErrorInvalidValue;
+  ffn::Arena ws{(char *)ws_ptr};
+  return (int)dispatch(*a, ws, true, (hipStream_t)stream, backward);
+}
+
+}  // namespace
+
+extern "C" {
+
+long butd_gated_ffn_ld_hidden(int dtype, int hidden) {
+  const long vec = dtype == BUTD_FFN_F32 ? 4 : 8;
+  return ((long)hidden + vec - 1) / vec * vec;
+}
+int butd_gated_ffn_set_tile(int tile, int split) {
+  if (tile == 0 && split == 0) {
+    ffn::forced_tile = ffn::forced_split = 0;
+    return 0;
+  }
+  if ((tile != 64 && tile != 128 && tile != 256) || split < 1 || split > 64) return (int)hipErrorInvalidValue;
+  ffn::forced_tile = tile;
+  ffn::forced_split = split;
+  return 0;
+}
+long butd_gated_ffn_fwd_workspace(const butd_gated_ffn_args *args) { return workspace(args, false); }
+long butd_gated_ffn_bwd_workspace(const butd_gated_ffn_args *args) { return workspace(args, true); }
+int butd_gated_ffn_fwd(const butd_gated_ffn_args *args, void *ws, long ws_bytes, butd_stream_t stream) {
+  return execute(args, ws, ws_bytes, stream, false);
+}
+int butd_gated_ffn_bwd(const butd_gated_ffn_args *args, void *ws, long ws_bytes, butd_stream_t stream) {
+  return execute(args, ws, ws_bytes, stream, true);
+}
+
+}  // extern "C"

@@ -1,0 +1,101 @@
+"""Norms around a block without a GPU: refusals, the stock-torch backend, the C entry points' checks."""
+import ctypes
+
+import pytest
+import torch
+from torch import nn
+
+
+def test_cpu_tensors_are_refused():
+    from butd_detr_amd.residual_norm import residual_norm
+    with pytest.raises(RuntimeError, match="CPU not supported"):
+        residual_norm(torch.randn(2, 3, 8), torch.randn(2, 3, 8), pre_norm=nn.LayerNorm(8))
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(x=torch.randn(2, 3, 8).double()), "not served"),
+    (dict(x=torch.tensor(1.0)), "cols"),
+    (dict(x=torch.randn(2, 3, 0)), "cols"),
+    (dict(x=torch.randn(1, 8193)), "rows of up to 8192"),
+    (dict(residual=torch.randn(2, 1, 8)), "residual must be"),
+    (dict(residual=torch.randn(2, 3, 8).half()), "residual must be"),
+    (dict(post_norm=nn.LayerNorm(4)), "must normalise"),
+    (dict(pre_norm=nn.LayerNorm((3, 8))), "must normalise"),
+    (dict(pre_norm=nn.BatchNorm1d(8)), "nn.LayerNorm or nn.RMSNorm"),
+    (dict(post_norm=nn.RMSNorm(8).half()), "must be torch.float32 or float32"),
+    (dict(gate=torch.randn(3, 8)), "gate must be"),
+    (dict(gate=torch.randn(2, 3, 1)), "gate must be"),
+    (dict(gate=torch.randn(8).half()), "gate must be"),
+])
+def test_refusals(change, message):
+    from butd_detr_amd.residual_norm import residual_norm
+    args = dict(x=torch.randn(2, 3, 8))
+    args.update(change)
+    with pytest.raises(RuntimeError, match=message):
+        residual_norm(**args)
+
+
+def test_torch_backend():
+    from butd_detr_amd import attention_blocks as ab
+    from butd_detr_amd.gated_ffn import GatedFeedForward
+    torch.manual_seed(0)
+    x, r = torch.randn(2, 3, 8), torch.randn(2, 3, 8)
+    post, pre, ffn = nn.RMSNorm(8), nn.LayerNorm(8), GatedFeedForward(8, 12)
+    prev = ab.get_backend()
+    try:
+        ab.set_backend("torch")
+        for gate in (None, torch.randn(8), torch.randn(2, 8), torch.randn(2, 3, 8)):
+            g = 1.0 if gate is None else gate[:, None] if gate.dim() == 2 else gate
+            stream, normed = ab.residual_norm(x, r, post_norm=post, gate=gate, residual_scale=0.5, pre_norm=pre)
+            torch.testing.assert_close(stream, 0.5 * r + g * post(x))
+            torch.testing.assert_close(normed, pre(stream))
+        assert ab.residual_norm(x)[1] is None
+        stream, normed = ab.gated_ffn_block(ffn, x, pre_norm=pre, post_norm=post, next_norm=pre)
+        torch.testing.assert_close(stream, x + post(ffn(pre(x))))
+        again, none = ab.gated_ffn_block(ffn, stream, normed=normed)
+        torch.testing.assert_close(again, stream + ffn(pre(stream)))
+        assert none is None
+        with pytest.raises(ValueError, match="one of"):
+            ab.gated_ffn_block(ffn, x)
+        with pytest.raises(ValueError, match="one of"):
+            ab.gated_ffn_block(ffn, x, pre_norm=pre, normed=x)
+    finally:
+        ab.set_backend(prev)
+
+
+def _filled():
+    from butd_detr_amd._hiplib import ResidualNormArgs
+    a = ResidualNormArgs()
+    a.x_dtype, a.stream_dtype, a.post_dtype, a.pre_dtype, a.gate_dtype = 1, 0, 1, 0, 1
+    a.post_kind, a.pre_kind, a.gate_kind = 1, 2, 2
+    a.rows, a.rows_per_sample, a.cols = 12, 4, 24
+    a.residual_scale, a.post_eps, a.pre_eps = 1.0, 1e-6, 1e-5
+    a.x, a.residual, a.gate, a.stream, a.normed, a.stats = (4096 * (i + 1) for i in range(6))     # never dereferenced
+    return a
+
+
+def test_entry_points_check_their_arguments():
+    from butd_detr_amd import _hiplib
+    lib = _hiplib.load()
+    need = lambda a: lib.butd_residual_norm_bwd_workspace(ctypes.byref(a))      # noqa: E731
+    a = _filled()
+    assert need(a) == 0
+    a.post_weight, a.d_post_weight, a.d_gate = 4096, 4096, 4096
+    assert need(a) > 0
+    assert lib.butd_residual_norm_bwd(ctypes.byref(a), None, 0, None) != 0
+    assert lib.butd_residual_norm_bwd(ctypes.byref(a), 4096, need(a) - 1, None) != 0
+    assert lib.butd_residual_norm_bwd(ctypes.byref(a), 4104, need(a), None) != 0
+    for field, value in [("x_dtype", 3), ("stream_dtype", 2), ("post_dtype", 2), ("gate_dtype", 2), ("post_kind", 3),
+                         ("pre_kind", -1), ("gate_kind", 4), ("rows", -1), ("rows", 1 << 31), ("rows_per_sample", 0),
+                         ("rows_per_sample", 5), ("cols", 0), ("cols", 8193), ("x", 0), ("x", 4097), ("gate", 0),
+                         ("residual", 4098), ("stream", 0), ("normed", 0)]:
+        a = _filled()
+        setattr(a, field, value)
+        assert lib.butd_residual_norm_fwd(ctypes.byref(a), None) != 0, field
+    for field, value in [("x", 0), ("cols", 0), ("rows_per_sample", 5), ("d_gate", 4097)]:
+        a = _filled()
+        setattr(a, field, value)
+        assert need(a) < 0, field
+    a = _filled()
+    a.stats = 0
+    assert need(a) < 0                                                          # the post norm's statistics are missing
