@@ -1,38 +1,75 @@
-"""Builds ``pointnet2_aten.cpp`` -- the ATen / pybind11 front end of the C ABI under the reference's module
-surface (``pointnet2._ext``, bindings.cpp:11-24) -- in-tree with torch.utils.cpp_extension:
+"""Builds the ATen / pybind11 front ends of the C ABI in-tree with torch.utils.cpp_extension:
 
-    python -m butd_detr_amd.binding.build          ->  butd_detr_amd/binding/_build/butd_pointnet2_aten.so
+    python -m butd_detr_amd.binding.build   ->  butd_detr_amd/binding/_build/butd_pointnet2_aten.so
+                                                butd_detr_amd/binding/_build/blocks/butd_blocks_aten.so
 
-Plain C++ (no device code): it links libbutd_detr_hip.so (``python -m butd_detr_amd.build``) and torch.
-The product path does not need it (it binds the same C ABI with ctypes); it exists so that the boundary is
-proven to bind where the reference's own shims (src/sampling.cpp:9-18 ...) would call it.
+Plain C++ (no device code): they link libbutd_detr_hip.so (``python -m butd_detr_amd.build``) and torch.
+
+* ``pointnet2_aten.cpp`` is the reference's module surface (``pointnet2._ext``, bindings.cpp:11-24).  The product path does
+  not need it (it binds the same C ABI with ctypes); it exists so that the boundary is proven to bind where the reference's
+  own shims (src/sampling.cpp:9-18 ...) would call it.
+* ``blocks_aten.cpp`` IS the path of ``gated_ffn`` and ``residual_norm``: their checks, allocations and autograd nodes.
 """
+import importlib.machinery
+import importlib.util
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 BUILD_DIR = os.path.join(HERE, "_build")
+BLOCKS_DIR = os.path.join(BUILD_DIR, "blocks")
 NAME = "butd_pointnet2_aten"
+BLOCKS = "butd_blocks_aten"
 
 
-def load(verbose=False):
-    """Compile (first call) and import the extension module."""
+def _compile(name, source, directory, verbose):
     import torch  # noqa: F401
     from torch.utils import cpp_extension
     from .. import build as libbuild
     lib_path = libbuild.build()
     lib_dir = os.path.dirname(lib_path)
-    os.makedirs(BUILD_DIR, exist_ok=True)
+    os.makedirs(directory, exist_ok=True)
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     return cpp_extension.load(
-        name=NAME, sources=[os.path.join(HERE, "pointnet2_aten.cpp")],
+        name=name, sources=[os.path.join(HERE, source)],
         extra_include_paths=[os.path.join(ROOT, "include"), os.path.join(rocm, "include")],
         extra_cflags=["-O2", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"],
         extra_ldflags=[f"-L{lib_dir}", "-lbutd_detr_hip", f"-Wl,-rpath,{lib_dir}",
                        f"-L{os.path.join(os.path.dirname(torch.__file__), 'lib')}", "-lc10_hip", "-ltorch_hip"],
-        build_directory=BUILD_DIR, with_cuda=False, verbose=verbose)
+        build_directory=directory, with_cuda=False, verbose=verbose)
+
+
+def load(verbose=False):
+    """Compile (first call) and import the reference's module surface."""
+    return _compile(NAME, "pointnet2_aten.cpp", BUILD_DIR, verbose)
+
+
+def compile_blocks(verbose=False):
+    """Compile what changed of the blocks' front end and import it."""
+    global _blocks
+    _blocks = _compile(BLOCKS, "blocks_aten.cpp", BLOCKS_DIR, verbose)
+    return _blocks
+
+
+_blocks = None
+
+
+def blocks():
+    """The blocks' front end as it was built; compiled only where nothing is built yet."""
+    global _blocks
+    if _blocks is None:
+        path = os.path.join(BLOCKS_DIR, BLOCKS + ".so")
+        if not os.path.exists(path):
+            return compile_blocks()
+        import torch  # noqa: F401
+        from .. import _hiplib
+        _hiplib.load()                         # (the library it links: missing -> says how to build it)
+        spec = importlib.util.spec_from_file_location(BLOCKS, path, loader=importlib.machinery.ExtensionFileLoader(BLOCKS, path))
+        _blocks = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_blocks)
+    return _blocks
 
 
 if __name__ == "__main__":
-    m = load(verbose=True)
-    print(m.__file__)
+    for m in (load(verbose=True), compile_blocks(verbose=True)):
+        print(m.__file__)
