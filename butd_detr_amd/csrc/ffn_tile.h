@@ -93,18 +93,18 @@ template <int KIND> __device__ inline void activation(float a, float &v, float &
     d = s * (1.f - s);
   }
 }
-template <int KIND> __device__ inline void activation4_of(const float *a, float *v, float *d) {
+template <int KIND, int N> __device__ inline void activations_of(const float *a, float *v, float *d) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) activation<KIND>(a[e], v[e], d[e]);
+  for (int e = 0; e < N; ++e) activation<KIND>(a[e], v[e], d[e]);
 }
-// four elements behind one uniform branch
-__device__ inline void activation4(int kind, const float *a, float *v, float *d) {
+// N elements behind one uniform branch
+template <int N> __device__ inline void activations(int kind, const float *a, float *v, float *d) {
   switch (kind) {
-    case kSilu: activation4_of<kSilu>(a, v, d); break;
-    case kGelu: activation4_of<kGelu>(a, v, d); break;
-    case kGeluTanh: activation4_of<kGeluTanh>(a, v, d); break;
-    case kRelu: activation4_of<kRelu>(a, v, d); break;
-    default: activation4_of<kSigmoid>(a, v, d);
+    case kSilu: activations_of<kSilu, N>(a, v, d); break;
+    case kGelu: activations_of<kGelu, N>(a, v, d); break;
+    case kGeluTanh: activations_of<kGeluTanh, N>(a, v, d); break;
+    case kRelu: activations_of<kRelu, N>(a, v, d); break;
+    default: activations_of<kSigmoid, N>(a, v, d);
   }
 }
 
@@ -128,12 +128,15 @@ struct Problem {
   float *slab;
   long slab_stride;
   int split;
-  int tiles_m, tiles_n, first; // first block of this problem
+  // filled in by the launch: tiles, the first block's x of this problem, steps of the contraction in all and of a slice,
+  // and 2^32 / (8 tiles_n) + 1
+  int tiles_m, tiles_n, first, steps, per_slice;
+  uint32_t group_magic;
 };
 constexpr int kMaxProblems = 3;
 struct Launch {
   Problem p[kMaxProblems];
-  int count, act, total;
+  int count, act, total;       // total: blocks in x; the slices are blocks in y
 };
 
 // blockIdx -> work item: the chip deals consecutive workgroups to its 8 dies in turn; the dies' L2 caches are separate, so
@@ -152,6 +155,8 @@ struct Config {
   static constexpr int kind = KIND, TM = TM_, TN = TN_, WM = WM_, WN = WN_, NW = WM_ * WN_;
   static constexpr bool a_kc = AK, b_kc = BK_;
   static constexpr int FM = TM / WM / 16, FN = TN / WN / 16;
+  static constexpr bool kMulti = KIND == kPlain && !AK;           // the weight gradients: several problems in a launch
+  static constexpr bool kSegments = KIND == kPlain && AK && !BK_; // dx: two contraction segments
   static constexpr int kA = TM * 128, kB = TN * 128;     // bytes of a stage
   static constexpr int kThreads = NW * 64;
 };
@@ -206,36 +211,37 @@ template <typename T, int EXT, int F, bool KC, bool PAIR>
 struct Reader {
   static constexpr int kRowBytes = EXT * (int)sizeof(T);
   static constexpr int kGroup = (!KC && sizeof(T) == 4) ? (F >= 4 ? 4 : F) : 1;
+  static constexpr int kReads = KC ? F : sizeof(T) == 2 ? 2 * F : 4 * F / kGroup;      // LDS instructions of one read()
   static_assert(F % kGroup == 0, "");
   int base;
-  int key;
   __device__ inline void init(int lane, int first) {     // first: first row of the wave's part of the tile
     const int i = lane & 15, g = lane >> 4;
     if constexpr (KC) {
       const int row = PAIR ? 8 * (i >> 2) + (i & 3) : i;
-      key = (PAIR ? key_pair(row) : key_natural(row));
-      base = (first + row) * 128 + ((g ^ key) << 4);     // step 1 flips bit 2 of the unit: address ^ 64
+      base = (first + row) * 128 + ((g ^ (PAIR ? key_pair(row) : key_natural(row))) << 4);     // step 1 flips bit 2 of the unit: address ^ 64
     } else if constexpr (sizeof(T) == 2) {
+      // granule of tile t: ((first >> 4) + t) ^ key, = ((first >> 4) ^ key) ^ t since t stays below the alignment of first
       const int k = 8 * g + (i >> 2);
-      key = key_pair(k) & (kRowBytes / 32 - 1);
-      base = k * kRowBytes + (i & 3) * 8;
+      base = k * kRowBytes + (i & 3) * 8 + (((first >> 4) ^ (key_pair(k) & (kRowBytes / 32 - 1))) << 5);
     } else {
       base = 4 * g * kRowBytes + (first + kGroup * i) * 4;
-      key = 0;
     }
   }
-  __device__ inline void read(const char *lds, int first, int s, u32x4 *frag) const {
+  __device__ inline void read(const char *lds, int s, u32x4 *frag) const {
     if constexpr (KC) {
+      int b = base ^ (s << 6);
 #pragma unroll
       for (int t = 0; t < F; ++t) {
         // PAIR: tiles 2 G, 2 G + 1 cover the rows 32 G + 8 (i / 4) + 4 (t % 2) + i % 4
         const int off = PAIR ? (t >> 1) * (32 * 128) + (t & 1) * (4 * 128) : t * (16 * 128);
-        frag[t] = *(const u32x4 *)(lds + (base ^ (s << 6)) + off);
+        frag[t] = *(const u32x4 *)(lds + b + off);
       }
     } else if constexpr (sizeof(T) == 2) {
+      int b = base;
+      asm volatile("" : "+v"(b));                        // (one XOR a tile here, not a register a tile across the loop)
 #pragma unroll
       for (int t = 0; t < F; ++t) {
-        const int addr = base + ((((first >> 4) + t) ^ key) << 5);
+        const int addr = b ^ (t << 5);
         u32x4 f;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
@@ -282,6 +288,17 @@ template <> __device__ inline void store_quad<_Float16>(_Float16 *p, const float
   *(v4 *)p = v4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
 }
 
+// ... through a buffer descriptor: dropped where the offset is out of its bound
+template <typename T> __device__ inline void store_buffer(__amdgpu_buffer_rsrc_t r, uint32_t off, const float *v) {
+  if constexpr (sizeof(T) == 4) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]}), r, off, 0, 0);
+  } else {
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]}), r, off, 0, 0);
+  }
+}
+
 // four consecutive columns n .. n + 3 of a row; `whole`: rows of this matrix start at vector boundaries
 template <typename T> __device__ inline void put(T *row, int n, int N, int pad, bool whole, const float *v) {
   if (whole && n + 4 <= N) {
@@ -308,23 +325,33 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
   __builtin_amdgcn_s_setprio(BUTD_MAIN_PRIO);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  // ---- which tile
-  const int item = die_local(blockIdx.x, L.total);
+  // ---- which tile.  (Divisions by run-time numbers cost hundreds of cycles each before the first load: the host's share of
+  // them comes with the arguments.)
+  const int item = die_local(blockIdx.x, L.total), slice = blockIdx.y;
   int pi = 0;
+  if constexpr (C::kMulti) {
 #pragma unroll
-  for (int i = 1; i < kMaxProblems; ++i)
-    if (i < L.count && item >= L.p[i].first) pi = i;
-  const Problem P = L.p[pi];                             // (a copy: scalar registers, not reloads behind every barrier)
-  const int local = item - P.first, tiles = P.tiles_m * P.tiles_n;
-  const int slice = local / tiles, idx = local - slice * tiles;
+    for (int i = 1; i < kMaxProblems; ++i)
+      if (i < L.count && item >= L.p[i].first) pi = i;
+  }
+  const Problem P = L.p[C::kMulti ? pi : 0];             // (a copy: scalar registers, not reloads behind every barrier)
+  if (C::kMulti && slice >= P.split) return;
+  const int idx = item - P.first;
   constexpr int kGroupM = 8;                             // 8 x n blocks of tiles: neighbours share both operands in L2
-  const int width = kGroupM * P.tiles_n, grp = idx / width, first_m = grp * kGroupM;
-  const int gsz = min(P.tiles_m - first_m, kGroupM), in = idx - grp * width;
-  const int m0 = (first_m + in % gsz) * C::TM, n0 = (in / gsz) * (C::TN / kParts);
+  const int width = kGroupM * P.tiles_n;
+  int grp = (int)(((uint64_t)(uint32_t)idx * P.group_magic) >> 32);              // idx / width, or one more
+  if (grp * width > idx) --grp;
+  const int first_m = grp * kGroupM, gsz = min(P.tiles_m - first_m, kGroupM), in = idx - grp * width;
+  int tn = in >> 3;                                      // in / gsz
+  if (gsz != kGroupM) {
+    tn = __builtin_amdgcn_readfirstlane((int)((float)in * __builtin_amdgcn_rcpf((float)gsz)));
+    const int rest = in - tn * gsz;
+    tn += rest < 0 ? -1 : rest >= gsz ? 1 : 0;
+  }
+  const int m0 = (first_m + in - tn * gsz) * C::TM, n0 = tn * (C::TN / kParts);
 
-  const int per_seg = (P.K + BK - 1) / BK, steps = per_seg * P.segments;
-  const int per_slice = (steps + P.split - 1) / P.split;
-  const int it0 = slice * per_slice, it1 = min(steps, it0 + per_slice);
+  const int per_seg = (P.K + BK - 1) / BK;
+  const int it0 = slice * P.per_slice, it1 = min(P.steps, it0 + P.per_slice);
 
   const int wm = wave / C::WN, wn = wave % C::WN;
   const int a_first = wm * (FM * 16), b_first = wn * (FP * 16);
@@ -332,13 +359,11 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
   Loader<T, C::TM, C::NW, C::a_kc, false> la;
   Loader<T, C::TN, C::NW, C::b_kc, kPairB> lb;
   la.init(wave, lane, P.lda);
+  lb.init(wave, lane, P.ldb);
   if constexpr (kParts == 2) {
     // rows TN/2 .. TN - 1 of the tile are W_up's rows 0 .. TN/2 - 1
-    lb.init(wave, lane, P.ldb);
 #pragma unroll
     for (int j = lb.kChunks / 2; j < lb.kChunks; ++j) lb.voff[j] -= (uint32_t)(C::TN / 2 * P.ldb);
-  } else {
-    lb.init(wave, lane, P.ldb);
   }
   Reader<T, C::TM, FM, C::a_kc, false> ra;
   Reader<T, C::TN, FP, C::b_kc, kPairB> rb;
@@ -374,18 +399,35 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
       b_bytes = (long)(left - 1) * P.ldb + unit_n;
     }
   };
-  seek(it0 >= per_seg ? 1 : 0, (it0 >= per_seg ? it0 - per_seg : it0) * BK);
+  if constexpr (C::kSegments) seek(it0 >= per_seg ? 1 : 0, (it0 >= per_seg ? it0 - per_seg : it0) * BK);
+  else seek(0, it0 * BK);
+  // (no branch around it: behind the last step nothing is readable, the stage arrives as zeros and costs no memory traffic)
   auto issue = [&](char *al, char *bl) {
-    la.issue(al, wave, pa, a_bytes, left);
+    const bool live = fetched < it1;
+    la.issue(al, wave, pa, live ? a_bytes : 0, left);
     if constexpr (kParts == 2) {
-      lb.issue(bl, wave, pb, b_bytes, left, 0, lb.kChunks / 2);
-      lb.issue(bl, wave, pb2, b_bytes, left, lb.kChunks / 2, lb.kChunks);
+      lb.issue(bl, wave, pb, live ? b_bytes : 0, left, 0, lb.kChunks / 2);
+      lb.issue(bl, wave, pb2, live ? b_bytes : 0, left, lb.kChunks / 2, lb.kChunks);
       pb2 += step_b;
     } else {
-      lb.issue(bl, wave, pb, b_bytes, left);
+      lb.issue(bl, wave, pb, live ? b_bytes : 0, left);
     }
-    pa += step_a; pb += step_b; a_bytes -= step_a; b_bytes -= step_b; left -= BK;
-    if (++fetched == per_seg) seek(1, 0);
+    pa += step_a;
+    pb += step_b;
+    a_bytes -= step_a;
+    b_bytes -= step_b;
+    left -= BK;
+    ++fetched;
+    if constexpr (C::kSegments) {
+      // the second segment has the first one's shape: back to its k = 0 on the other pointers
+      const bool over = fetched == per_seg;
+      const long back = (long)per_seg * BK;
+      pa = over ? (const char *)P.a[1] + (long)m0 * P.lda : pa;
+      pb = over ? (const char *)P.b[1] + (long)n0 * (int)sizeof(T) : pb;
+      a_bytes += over ? back * (int)sizeof(T) : 0;
+      b_bytes += over ? back * P.ldb : 0;
+      left += over ? (int)back : 0;
+    }
   };
 
   f32x4 acc[FM][FN];
@@ -400,8 +442,8 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
   u32x4 fa[2][FM], fb[2][FN];
   auto read = [&](const char *al, const char *bl, int s) {
 #pragma unroll
-    for (int q = 0; q < kParts; ++q) rb.read(bl + q * (C::TN / 2 * 128), b_first, s, fb[s] + q * FP);
-    ra.read(al, a_first, s, fa[s]);
+    for (int q = 0; q < kParts; ++q) rb.read(bl + q * (C::TN / 2 * 128), s, fb[s] + q * FP);
+    ra.read(al, s, fa[s]);
   };
   auto multiply = [&](int s) {
 #pragma unroll
@@ -418,28 +460,46 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
     asm volatile("s_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  if (it0 < it1) {
-    issue(a_lds0, b_lds0);
-    fence();
-    if (it0 + 1 < it1) issue(a_lds1, b_lds1);
-    read(a_lds0, b_lds0, 0);
-  }
-  // (one exit: a break behind the first half made the compiler keep a second copy of the accumulators)
-  for (int it = it0; it < it1; it += 2) {
-    read(a_lds0, b_lds0, 1);
-    multiply(0);
-    fence();
-    if (it + 2 < it1) issue(a_lds0, b_lds0);
-    if (it + 1 < it1) read(a_lds1, b_lds1, 0);
-    multiply(1);
-    if (it + 1 < it1) {
-      read(a_lds1, b_lds1, 1);
-      multiply(0);
-      fence();
-      if (it + 3 < it1) issue(a_lds1, b_lds1);
-      if (it + 2 < it1) read(a_lds0, b_lds0, 0);
-      multiply(1);
+  // The order of a half's instructions: a wave issues in order, and a run of LDS reads in front of the matrix instructions
+  // holds those back while the LDS works the run off.  One direct load or read behind every matrix instruction hides both:
+  // 3150 -> 2720 cycles a stage (4096^3, 256 tile; 2048 are the matrix instructions'), whichever side is K-strided.  Two
+  // workgroups of the 128 tile share a CU and cover for each other; ordered like this they lose 10 %.
+  constexpr bool kInterleave = C::NW == 8;
+  constexpr int kReads = decltype(ra)::kReads + kParts * decltype(rb)::kReads, kLoads = decltype(la)::kChunks + decltype(lb)::kChunks;
+  auto interleave = [&](int loads) {
+    if constexpr (kInterleave) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        if (i >= loads) break;
+        __builtin_amdgcn_sched_group_barrier(0x020, 1, 0); // direct load
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // matrix instruction
+      }
+#pragma unroll
+      for (int i = 0; i < kReads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); // LDS read
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
     }
+  };
+  // both halves of the stage in (al, bl); (an, bn): the other stage, which is on its way
+  auto stage = [&](char *al, char *bl, const char *an, const char *bn) {
+    read(al, bl, 1);
+    multiply(0);
+    interleave(0);
+    fence();
+    issue(al, bl);
+    read(an, bn, 0);
+    multiply(1);
+    interleave(kLoads);
+  };
+  issue(a_lds0, b_lds0);
+  fence();
+  issue(a_lds1, b_lds1);
+  read(a_lds0, b_lds0, 0);
+  // (one exit: a break behind the first stage made the compiler keep a second copy of the accumulators)
+  for (int it = it0; it < it1; it += 2) {
+    stage(a_lds0, b_lds0, a_lds1, b_lds1);
+    if (it + 1 < it1) stage(a_lds1, b_lds1, a_lds0, b_lds0);
   }
 
   // ---- epilogue.  The accumulators pass through LDS, a wave's own part of it, up to 64 of its rows at a time: behind that a
@@ -450,14 +510,128 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
   constexpr int kChunkBytes = CT * 16 * kCols * 4;
   static_assert(C::kA == C::kB && C::kA % kChunkBytes == 0 && kChunkBytes * C::NW <= 4 * C::kA, "");
   static_assert(FM % CT == 0 && CT % WA == 0 && (kQuads & (kQuads - 1)) == 0, "");
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");               // the last stage has been read by every wave
+  fence();                                               // every wave has read its last stage; no direct load is in flight
   const int slot = wave * kChunkBytes / C::kA;
   char *mine = (slot == 0 ? a_lds0 : slot == 1 ? b_lds0 : slot == 2 ? a_lds1 : b_lds1) + wave * kChunkBytes % C::kA;
   const int i16 = lane & 15, g = lane >> 4;
   const bool whole = (P.ldc % 4 == 0) && ((uintptr_t)P.c & 15) == 0 && ((uintptr_t)P.c2 & 15) == 0;
   const bool to_slab = C::kind == kPlain && P.split > 1;
+  constexpr int kLanes = kQuads / kParts, kRows = 64 / kLanes;                    // lanes of a row, rows of a step
+  constexpr int kSteps = CT * 16 / kRows, U = kSteps < 4 ? kSteps : 4;            // steps of a chunk, of a batch
+  static_assert(kSteps % U == 0, "");
+  static_assert((U * kRows) % 8 == 0, "a batch must not change the swizzle (quad ^ row % 8)");
+  const int quad = lane % kLanes, r_lane = lane / kLanes;
+  const int n = n0 + b_first + 4 * quad;
+  const uint32_t row_step = kRows;
+  // LDS address of step u of a batch (rows that are a multiple of the swizzle apart share it)
+  int place[U][kParts];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      const int r = u * kRows + r_lane;
+      place[u][part] = r * (kCols * 4) + (((part * kLanes + quad) ^ (r & 7)) << 4);
+    }
+  float bias0[4], bias1[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    bias0[e] = P.bias0 && n + e < P.N && !to_slab ? (float)((const T *)P.bias0)[n + e] : 0.f;
+    bias1[e] = kParts == 2 && P.bias1 && n + e < P.N ? (float)((const T *)P.bias1)[n + e] : 0.f;
+  }
+  // Whole rows of vectors (every column in one, rows at vector boundaries, no padding): buffer stores with 32-bit offsets;
+  // rows behind the last and columns behind N fall outside the descriptor's bound and are dropped.  Anything else goes
+  // element by element through put().
+  using OutT = T;
+  const bool vectors = (P.N & 3) == 0 && P.pad <= P.N && (to_slab || whole);
+  const long ld_out = to_slab ? P.N : P.ldc;
+  const int size_out = to_slab ? 4 : (int)sizeof(OutT);
+  const int m_base = m0 + a_first;
+  const auto bound = [&](long ld, int size) -> uint32_t {               // bytes from (m_base, 0) to the last column of the last row
+    const long bytes = ((long)(P.M - m_base - 1) * ld + P.N) * size;
+    return P.M <= m_base ? 0u : bytes > 0x7fffffffL ? 0x7fffffffu : (uint32_t)bytes;
+  };
+  const auto resource = [&](const void *base, long ld, int size) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)((const char *)base + (long)m_base * ld * size), 0, bound(ld, size), 0x00020000);
+  };
+  const __amdgpu_buffer_rsrc_t rc = to_slab ? resource(P.slab + (long)slice * P.slab_stride, ld_out, 4) : resource(P.c, ld_out, size_out);
+  __amdgpu_buffer_rsrc_t rc2 = rc, rx0 = rc, rx1 = rc;
+  if constexpr (C::kind == kGrad) {
+    rc2 = resource(P.c2, P.ldc, sizeof(T));
+    rx0 = resource(P.aux0, P.ldaux, 4);
+    rx1 = resource(P.aux1, P.ldaux, 4);
+  } else if constexpr (C::kind == kGateUp) {
+    rx0 = resource(P.out0, P.ldaux, 4);
+    rx1 = resource(P.out1, P.ldaux, 4);
+  }
+  const bool exists = n < P.N;
+  const uint32_t step_out = row_step * (uint32_t)(ld_out * size_out), step_aux = row_step * (uint32_t)(P.ldaux * 4);
+  const uint32_t off_out = exists ? (uint32_t)(r_lane * ld_out + n) * size_out : 0x80000000u;
+  const uint32_t off_aux = exists ? (uint32_t)(r_lane * P.ldaux + n) * 4 : 0x80000000u;
+
+  // what a batch reads from memory (kGrad: a and b); fetched one batch ahead, the first before the accumulators are staged
+  struct Aux {
+    f32x4 a[U], b[U];
+  };
+  auto fetch = [&](int step, Aux &x) {                   // step: counted over all chunks
+    if constexpr (C::kind == kGrad) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (vectors) {
+          const uint32_t off = off_aux + (step + u) * step_aux;
+          x.a[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx0, off, 0, 0));
+          x.b[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx1, off, 0, 0));
+        } else {
+          const int m = m_base + (step + u) * kRows + r_lane;
+          x.a[u] = x.b[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (m < P.M && n + e < P.N) {
+              x.a[u][e] = P.aux0[(long)m * P.ldaux + n + e];
+              x.b[u][e] = P.aux1[(long)m * P.ldaux + n + e];
+            }
+        }
+      }
+    }
+  };
+  // element-wise part of a batch: v (kParts x 4 of each step) -> o0, o1
+  auto combine = [&](float (&v)[U][kParts][4], const Aux &x, float (&o0)[U][4], float (&o1)[U][4]) {
+    if constexpr (C::kind == kPlain) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o0[u][e] = v[u][0][e] + bias0[e];
+    } else {
+      float a[U * 4], value[U * 4], slope[U * 4];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (C::kind == kGateUp) {
+            v[u][0][e] += bias0[e];
+            v[u][kParts - 1][e] += bias1[e];
+            a[u * 4 + e] = v[u][0][e];
+          } else {
+            a[u * 4 + e] = x.a[u][e];
+          }
+        }
+      activations<U * 4>(L.act, a, value, slope);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (C::kind == kGateUp) {
+            o0[u][e] = value[u * 4 + e] * v[u][kParts - 1][e];
+          } else {
+            o0[u][e] = v[u][0][e] * x.b[u][e] * slope[u * 4 + e];
+            o1[u][e] = v[u][0][e] * value[u * 4 + e];
+          }
+        }
+    }
+  };
 #pragma unroll
   for (int chunk = 0; chunk < FM / CT; ++chunk) {
+    Aux next;
+    fetch(chunk * kSteps, next);
 #pragma unroll
     for (int tt = 0; tt < CT; ++tt) {
       const int row = 16 * WA * (tt / WA) + WA * i16 + tt % WA;
@@ -474,78 +648,57 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
           const int c = 4 * (qq % WB) + e;               // column c = WB * r + tile of the group (WB == 1: the tile's own rows r)
           v[e] = acc[chunk * CT + tt][part * FP + (qq / WB) * WB + c % WB][c / WB];
         }
-        const int quad = part * (FP * 4) + (col >> 2);
-        *(f32x4 *)(mine + row * (kCols * 4) + ((quad ^ (row & (kQuads - 1))) << 4)) = v;
+        const int at = part * (FP * 4) + (col >> 2);
+        *(f32x4 *)(mine + row * (kCols * 4) + ((at ^ (row & 7)) << 4)) = v;
       }
     }
     // (a wave's own LDS traffic is in order: the reads below see the writes above without a barrier)
     asm volatile("" ::: "memory");
-    constexpr int kLanes = kQuads / kParts, kRows = 64 / kLanes;                  // lanes of a row, rows of a step
-    const int quad = lane % kLanes;
-    const int n = n0 + b_first + 4 * quad;
-#pragma unroll 2
-    for (int r = lane / kLanes; r < CT * 16; r += kRows) {
-      float v[kParts][4];
+#pragma unroll 1
+    for (int step = 0; step < kSteps; step += U) {
+      const Aux now = next;
+      if (step + U < kSteps) fetch(chunk * kSteps + step + U, next);
+      float v[U][kParts][4], o0[U][4], o1[U][4];
 #pragma unroll
-      for (int part = 0; part < kParts; ++part) {
-        const f32x4 w = *(const f32x4 *)(mine + r * (kCols * 4) + (((part * kLanes + quad) ^ (r & (kQuads - 1))) << 4));
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[part][e] = w[e];
-      }
-      const int m = m0 + a_first + chunk * (CT * 16) + r;
-      if (m >= P.M) continue;
-      if (to_slab) {
-        put<float>(P.slab + (long)slice * P.slab_stride + (long)m * P.N, n, P.N, 0, (P.N & 3) == 0, v[0]);
-        continue;
-      }
-      T *row = (T *)P.c + (long)m * P.ldc;
-      if constexpr (C::kind == kGateUp) {
-        float h[4];
+        for (int part = 0; part < kParts; ++part) {
+          const f32x4 w = *(const f32x4 *)(mine + place[u][part] + step * (kRows * kCols * 4));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (P.bias0 && n + e < P.N) v[0][e] += (float)((const T *)P.bias0)[n + e];
-          if (P.bias1 && n + e < P.N) v[1][e] += (float)((const T *)P.bias1)[n + e];
+          for (int e = 0; e < 4; ++e) v[u][part][e] = w[e];
         }
-        float slope[4];
-        activation4(L.act, v[0], h, slope);
+      combine(v, now, o0, o1);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) h[e] *= v[1][e];
-        put<T>(row, n, P.N, P.pad, whole, h);
-        if (P.out0) {
-          // kept in 32 bits: rounded to the operands' 16 bits here, the gradients of x and W_gate would carry two
-          // roundings more than the product's own operands do
-          put<float>(P.out0 + (long)m * P.ldaux, n, P.N, 0, true, v[0]);
-          put<float>(P.out1 + (long)m * P.ldaux, n, P.N, 0, true, v[1]);
-        }
-      } else if constexpr (C::kind == kGrad) {
-        f32x4 a4 = {0.f, 0.f, 0.f, 0.f}, b4 = a4;
-        if (n + 4 <= P.N) {
-          a4 = *(const f32x4 *)(P.aux0 + (long)m * P.ldaux + n);
-          b4 = *(const f32x4 *)(P.aux1 + (long)m * P.ldaux + n);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < P.N) {
-              a4[e] = P.aux0[(long)m * P.ldaux + n + e];
-              b4[e] = P.aux1[(long)m * P.ldaux + n + e];
+      for (int u = 0; u < U; ++u) {
+        const int done = chunk * kSteps + step + u;
+        if (vectors) {
+          const uint32_t off = off_out + done * step_out;
+          if (to_slab) store_buffer<float>(rc, off, o0[u]);
+          else store_buffer<T>(rc, off, o0[u]);
+          if constexpr (C::kind == kGrad) store_buffer<T>(rc2, off, o1[u]);
+          if constexpr (C::kind == kGateUp) {
+            if (P.out0) {
+              // kept in 32 bits: rounded to the operands' 16 bits here, the gradients of x and W_gate would carry two
+              // roundings more than the product's own operands do
+              const uint32_t aux = off_aux + done * step_aux;
+              store_buffer<float>(rx0, aux, v[u][0]);
+              store_buffer<float>(rx1, aux, v[u][kParts - 1]);
             }
+          }
+        } else {
+          const int m = m_base + done * kRows + r_lane;
+          if (m >= P.M) continue;
+          T *row = (T *)P.c + (long)m * P.ldc;
+          if (to_slab) put<float>(P.slab + (long)slice * P.slab_stride + (long)m * P.N, n, P.N, 0, false, o0[u]);
+          else put<T>(row, n, P.N, P.pad, whole, o0[u]);
+          if constexpr (C::kind == kGrad) put<T>((T *)P.c2 + (long)m * P.ldc, n, P.N, P.pad, whole, o1[u]);
+          if constexpr (C::kind == kGateUp) {
+            if (P.out0) {
+              put<float>(P.out0 + (long)m * P.ldaux, n, P.N, 0, true, v[u][0]);
+              put<float>(P.out1 + (long)m * P.ldaux, n, P.N, 0, true, v[u][kParts - 1]);
+            }
+          }
         }
-        float a[4] = {a4[0], a4[1], a4[2], a4[3]}, value[4], slope[4], da[4], db[4];
-        activation4(L.act, a, value, slope);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          da[e] = v[0][e] * b4[e] * slope[e];
-          db[e] = v[0][e] * value[e];
-        }
-        put<T>(row, n, P.N, P.pad, whole, da);
-        put<T>((T *)P.c2 + (long)m * P.ldc, n, P.N, P.pad, whole, db);
-      } else {
-        if (P.bias0) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < P.N) v[0][e] += (float)((const T *)P.bias0)[n + e];
-        }
-        put<T>(row, n, P.N, P.pad, whole, v[0]);
       }
     }
     asm volatile("" ::: "memory");

@@ -8,7 +8,7 @@
 namespace ffn {
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------
-// Up to 64 rows: the product reads every weight once and little else, so it is a stream of weights with 16 rows (a matrix
+// Up to 16 rows, and up to 64 with small weights: the product reads every weight once and little else, so it is a stream of weights with 16 rows (a matrix
 // instruction's width) per accumulator tile.  A workgroup owns 16 output columns; its waves share out the contraction in
 // 128-byte pieces (whole lines of the weights' rows), load straight into fragments -- nothing is reused between waves, LDS
 // would only add a trip -- and join their sums in LDS.
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(NW * 64) void few_rows_kernel(const FewRows P) {
   const bool whole = (P.ldc & 3) == 0 && ((uintptr_t)P.c & 15) == 0;
   if constexpr (PARTS == 2) {
     float h[4], slope[4];
-    activation4(P.act, v[0], h, slope);
+    activations<4>(P.act, v[0], h, slope);
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] *= v[1][e];
     put<T>(row, n, P.N, P.pad, whole, h);
@@ -159,14 +159,16 @@ struct Fold {
   const void *bias;
   long first;
 };
+constexpr int kMaxFolds = 2 * kMaxProblems;
 struct Folds {
-  Fold f[kMaxProblems];
+  Fold f[kMaxFolds];
   int count;
+  long blocks;
 };
 template <typename T> __global__ __launch_bounds__(256) void fold_kernel(const Folds L) {
   int fi = 0;
 #pragma unroll
-  for (int i = 1; i < kMaxProblems; ++i)
+  for (int i = 1; i < kMaxFolds; ++i)
     if (i < L.count && (long)blockIdx.x >= L.f[i].first) fi = i;
   const Fold F = L.f[fi];
   const long quads = (F.N + 3) / 4, q = ((long)blockIdx.x - F.first) * 256 + threadIdx.x;
@@ -177,10 +179,12 @@ template <typename T> __global__ __launch_bounds__(256) void fold_kernel(const F
   float v[4] = {0.f, 0.f, 0.f, 0.f};
   if ((F.N & 3) == 0) {
     f32x4 s = *(const f32x4 *)src;
+#pragma unroll 8
     for (int i = 1; i < F.split; ++i) s += *(const f32x4 *)(src + i * F.stride);      // in slice order: reproducible
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = s[e];
   } else {
+#pragma unroll 4
     for (int i = 0; i < F.split; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -194,7 +198,7 @@ template <typename T> __global__ __launch_bounds__(256) void fold_kernel(const F
   put<T>((T *)F.c + m * F.ldc, n, F.N, 0, (F.ldc & 3) == 0 && ((uintptr_t)F.c & 15) == 0, v);
 }
 
-// ---- bias gradients -------------------------------------------------------------------------------------------------------
+// ---- bias gradients: sums over chunks of rows, folded like slabs -------------------------------------------------------------
 struct ColumnSum {
   const void *src;
   long ld;                     // elements
@@ -228,23 +232,6 @@ template <typename T> __global__ __launch_bounds__(256) void column_sum_kernel(c
   if (sub == 0 && col < C.cols)
     C.part[(long)blockIdx.y * C.cols + col] = (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
 }
-template <typename T> __global__ __launch_bounds__(256) void column_sum_fold_kernel(const ColumnSums L) {
-  int ci = 0;
-#pragma unroll
-  for (int i = 1; i < 3; ++i)
-    if (i < L.count && (int)blockIdx.x >= L.c[i].first) ci = i;
-  const ColumnSum C = L.c[ci];
-  const int lane = threadIdx.x & 63, sub = threadIdx.x >> 6;
-  const int col = ((int)blockIdx.x - C.first) * 64 + lane;
-  float s = 0.f;
-  if (col < C.cols)
-    for (int k = sub; k < L.chunks; k += 4) s += C.part[(long)k * C.cols + col];
-  __shared__ float sums[4][64];
-  sums[sub][lane] = s;
-  __syncthreads();
-  if (sub == 0 && col < C.cols) ((T *)C.out)[col] = (T)((sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]));
-}
-
 // ---- plan -----------------------------------------------------------------------------------------------------------------
 constexpr int kCUs = 256;
 constexpr long kMaxLd = 1L << 22;      // bytes between rows: 256 rows of a tile stay within a buffer descriptor's 2 GB
@@ -263,61 +250,93 @@ enum Layout { kNT, kNN, kTN };         // A and B K-contiguous; B K-strided; bot
 
 struct TileChoice {
   int size, split;                     // 256, 128 or 64
+  double us;                           // modelled
 };
 
 // butd_gated_ffn_set_tile: (0, 0) = the rule below
 extern int forced_tile, forced_split;
 
-// Which tile, and into how many slices the contraction is cut (products whose slabs can be folded only).  Modelled time: the
-// tiles of a launch go round the chip in ceil(tiles / 256) turns (one tile per CU and turn), each turn costs the tile's
-// multiplications at the rate measured for that tile; slabs are written and read once at about 4 TB/s plus one launch.
+// Which tile, and into how many slices the contraction is cut (products whose slabs can be folded only): the smallest of the
+// modelled times.  The tiles go round the chip in batches of 256 CUs x as many workgroups as a CU holds.  A step of a batch
+// takes what one workgroup's step takes alone (latency) or what the multiplications of all workgroups of a CU take,
+// whichever is more; `fill` steps pass before the first and behind the last; the epilogue's bytes take the memory's time,
+// hidden in part where another workgroup of the CU computes meanwhile.  Slabs are written and read once, plus a launch.
+// No launch is faster than its operands' bytes at 4.5 TB/s.  Constants fitted to 120 measured launches of 16 shapes
+// (1 .. 8192 rows x 200 .. 4096 x 256 .. 11264, both widths of types): the chosen tile was the fastest one in 3 of 4 and at
+// most 18 % slower in the rest.
 struct Shape {
   long M, N;
 };
-template <typename T> inline TileChoice choose(const Shape *shapes, int count, long k, bool can_split) {
-  // multiply-adds per CU and microsecond at full occupancy, large sizes (see the table at the launches)
-  static const double rate16[3] = {2.2e6, 1.6e6, 0.8e6}, rate32[3] = {0, 0.22e6, 0.17e6};
-  const double *rate = sizeof(T) == 2 ? rate16 : rate32;
-  static const int sizes[3] = {256, 128, 64};
-  if (forced_tile) return TileChoice{sizeof(T) == 4 && forced_tile == 256 ? 128 : forced_tile, can_split ? forced_split : 1};
-  TileChoice best{64, 1};
-  double best_us = 1e30;
-  for (int c = 0; c < 3; ++c) {
-    if (rate[c] == 0) continue;
-    const int t = sizes[c];
+struct TileModel {
+  int size;
+  double latency_us, rate, fill;       // rate: multiply-adds per CU and microsecond with all CUs at work
+  int resident;                        // workgroups of a CU
+};
+template <typename T> inline TileChoice choose(const Shape *shapes, int count, long k, int segments, bool can_split, double epilogue_bytes) {
+  if (forced_tile) return TileChoice{sizeof(T) == 4 && forced_tile == 256 ? 128 : forced_tile, can_split ? forced_split : 1, 0.0};
+  static const TileModel models16[3] = {{64, 0.49, 1.15e6, 2.0, 4}, {128, 0.65, 1.75e6, 3.0, 2}, {256, 1.2, 2.4e6, 3.0, 1}};
+  static const TileModel models32[2] = {{64, 0.60, 0.245e6, 1.5, 4}, {128, 2.0, 0.258e6, 1.5, 2}};
+  static const int splits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+  const TileModel *models = sizeof(T) == 2 ? models16 : models32;
+  constexpr int bk = Num<T>::kBK;
+  const long steps = (k + bk - 1) / bk * segments;
+  TileChoice best{64, 1, 1e30};
+  double operands = 0;
+  for (int i = 0; i < count; ++i) operands += (double)(shapes[i].M + shapes[i].N) * (double)k * segments * sizeof(T);
+  for (int c = 0; c < (sizeof(T) == 2 ? 3 : 2); ++c) {
+    const TileModel &m = models[c];
+    const double area = (double)m.size * m.size, resident = kCUs * m.resident;
     double tiles = 0, elems = 0;
     for (int i = 0; i < count; ++i) {
-      tiles += (double)((shapes[i].M + t - 1) / t) * (double)((shapes[i].N + t - 1) / t);
+      tiles += (double)((shapes[i].M + m.size - 1) / m.size) * (double)((shapes[i].N + m.size - 1) / m.size);
       elems += (double)shapes[i].M * (double)shapes[i].N;
     }
-    for (int s = 1; s <= 64; s *= 2) {
-      if (s > 1 && (!can_split || k / s < 4 * Num<T>::kBK)) break;
-      const double turns = (double)(long)((tiles * s + kCUs - 1) / kCUs);
-      double us = turns * t * t * ((double)k / s + 2 * Num<T>::kBK) / rate[c];
-      if (s > 1) us += 3.0 + elems * 4 * (s + 1) / 4e6;
-      if (us < best_us) {
-        best_us = us;
-        best = TileChoice{t, s};
-      }
+    for (int s : splits) {
+      if (s > 1 && (!can_split || steps < 3L * s)) break;
+      const double turn = (double)((steps + s - 1) / s) + m.fill, bytes = s == 1 ? epilogue_bytes : 4.0;
+      const double all = tiles * s, full = (double)(long)(all / resident);
+      auto batch = [&](double workgroups) {
+        // a CU with one workgroup more than the others sets the time; with part of the chip idle the 16-bit matrix cores
+        // clock higher
+        const double per_cu = workgroups / kCUs, most = (double)(long)(per_cu + 0.999);
+        const double step = most * area * bk / m.rate * (sizeof(T) == 4 ? 1.0 : 0.6 + 0.4 * per_cu / most);
+        return turn * (step > m.latency_us ? step : m.latency_us) + per_cu * area * bytes / 2e4 * (m.resident == 1 ? 1.2 : 0.6);
+      };
+      double us = 3.0 + full * batch(resident);
+      if (all > full * resident) us += batch(all - full * resident);
+      if (us < 3.0 + operands / 4.5e6) us = 3.0 + operands / 4.5e6;
+      if (s > 1) us += 3.5 + elems * (4.0 * s + sizeof(T)) / 4.5e6;
+      if (us < best.us) best = TileChoice{m.size, s, us};
     }
   }
   return best;
 }
 
+// The streaming kernel's time: the weights once, and the rows again for every 16 columns (from L2; padded to 32 or 64).
+template <typename T> inline double few_rows_us(long M, long N, long K, int parts) {
+  const double rows = M <= 32 ? 32 : 64;
+  return 3.0 + (double)N * K * sizeof(T) * parts / 5.6e6 + rows / 16 * (double)N * K * sizeof(T) / 6.5e6;
+}
+
 template <class C> inline hipError_t launch_tiles(Launch &L, hipStream_t stream) {
+  constexpr int nw = C::kind == kGateUp ? C::TN / 2 : C::TN, bk = Num<typename C::type>::kBK;
   long total = 0;
-  constexpr int nw = C::kind == kGateUp ? C::TN / 2 : C::TN;
+  int slices = 1;
   for (int i = 0; i < L.count; ++i) {
     Problem &p = L.p[i];
     const long tm = ((long)p.M + C::TM - 1) / C::TM, tn = ((long)p.N + nw - 1) / nw;
-    if (tm * tn * p.split > 0x7fffffffL - total) return hipErrorInvalidValue;
+    if (tm * tn > 0x7fffffffL - total) return hipErrorInvalidValue;
     p.tiles_m = (int)tm;
     p.tiles_n = (int)tn;
     p.first = (int)total;
-    total += tm * tn * p.split;
+    p.steps = (int)(((long)p.K + bk - 1) / bk) * p.segments;
+    p.per_slice = (p.steps + p.split - 1) / p.split;
+    p.group_magic = (uint32_t)((1ULL << 32) / (8ULL * (uint64_t)tn)) + 1;
+    total += tm * tn;
+    if (p.split > slices) slices = p.split;
   }
   L.total = (int)total;
-  hipLaunchKernelGGL((tile_kernel<C>), dim3((unsigned)total), dim3(C::kThreads), 0, stream, L);
+  hipLaunchKernelGGL((tile_kernel<C>), dim3((unsigned)total, (unsigned)slices), dim3(C::kThreads), 0, stream, L);
   return hipGetLastError();
 }
 
@@ -374,9 +393,13 @@ template <typename T> struct Block {
       return hipGetLastError();
     }
   };
+  static bool direct_pair(const butd_gated_ffn_args &A) {
+    return A.ld_gate == A.ld_up && Packer::direct(A.w_gate, A.ld_gate, A.width) && Packer::direct(A.w_up, A.ld_up, A.width);
+  }
+  static bool direct_in(const butd_gated_ffn_args &A) { return direct_pair(A) && Packer::direct(A.x, A.ld_x, A.width); }
   // the two projections share one row stride in the product
   static void take_pair(Packer &pk, const butd_gated_ffn_args &A, Operand &gate, Operand &up) {
-    if (A.ld_gate == A.ld_up && Packer::direct(A.w_gate, A.ld_gate, A.width) && Packer::direct(A.w_up, A.ld_up, A.width)) {
+    if (direct_pair(A)) {
       gate = Operand{A.w_gate, A.ld_gate};
       up = Operand{A.w_up, A.ld_up};
     } else {
@@ -392,20 +415,26 @@ template <typename T> struct Block {
     p.segments = 1;
     p.split = 1;
   }
-  static hipError_t fold(const Launch &L, hipStream_t stream) {
-    Folds F;
-    F.count = 0;
-    long blocks = 0;
+  static void add_fold(Folds &F, const float *slab, long stride, int split, int M, int N, void *c, long ldc, const void *bias) {
+    F.f[F.count++] = Fold{slab, stride, split, M, N, c, ldc, bias, F.blocks};
+    F.blocks += ((long)M * ((N + 3) / 4) + 255) / 256;
+  }
+  static void add_folds(Folds &F, const Launch &L) {
     for (int i = 0; i < L.count; ++i) {
       const Problem &p = L.p[i];
-      if (p.split == 1) continue;
-      F.f[F.count++] = Fold{p.slab, p.slab_stride, p.split, p.M, p.N, p.c, p.ldc, p.bias0, blocks};
-      blocks += ((long)p.M * ((p.N + 3) / 4) + 255) / 256;
+      if (p.split > 1) add_fold(F, p.slab, p.slab_stride, p.split, p.M, p.N, p.c, p.ldc, p.bias0);
     }
+  }
+  static hipError_t run_folds(const Folds &F, hipStream_t stream) {
     if (!F.count) return hipSuccess;
-    if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((fold_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, F);
+    if (F.blocks > 0x7fffffffL) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((fold_kernel<T>), dim3((unsigned)F.blocks), dim3(256), 0, stream, F);
     return hipGetLastError();
+  }
+  static hipError_t fold(const Launch &L, hipStream_t stream) {
+    Folds F{};
+    add_folds(F, L);
+    return run_folds(F, stream);
   }
   static void slabs(Launch &L, int split, Arena &ws) {
     for (int i = 0; i < L.count; ++i) {
@@ -441,38 +470,54 @@ template <typename T> struct Block {
     const int M = (int)A.rows, E = A.width, F = A.hidden;
     if (M == 0) return hipSuccess;
     hipError_t err;
-    if (M <= kFewRows) {
-      if (!run) return hipSuccess;
-      FewRows P{A.x, A.w_gate, A.w_up, A.ld_x, A.ld_gate, A.ld_up, M, F, E, A.activation, A.h, A.ld_h, (int)A.ld_h,
-                A.b_gate, A.b_up, A.a, A.b, A.ld_h};
-      if ((err = few_rows<2>(P, stream)) != hipSuccess) return err;
-      FewRows D{A.h, A.w_down, A.w_down, A.ld_h, A.ld_down, A.ld_down, M, E, F, A.activation, A.y, A.ld_y, 0,
-                A.b_down, nullptr, nullptr, nullptr, 0};
-      return few_rows<1>(D, stream);
-    }
-    Packer pk(ws);
-    Operand x = pk.take(A.x, A.ld_x, M, E), gate, up;
-    take_pair(pk, A, gate, up);
-    Operand down = pk.take(A.w_down, A.ld_down, E, F);
-    Launch G{}, D{};
-    G.count = D.count = 1;
-    G.act = D.act = A.activation;
-    Problem &g = G.p[0], &d = D.p[0];
-    operands(g, x, gate);
-    g.b[1] = up.p;
-    g.M = M; g.N = F; g.K = E;
-    g.c = A.h; g.ldc = A.ld_h; g.pad = (int)A.ld_h;
-    g.bias0 = A.b_gate; g.bias1 = A.b_up;
-    g.out0 = A.a; g.out1 = A.b; g.ldaux = A.ld_h;
-    operands(d, Operand{A.h, A.ld_h}, down);
-    d.M = M; d.N = E; d.K = F;
-    d.c = A.y; d.ldc = A.ld_y; d.bias0 = A.b_down;
+    // Each product of up to 16 rows is streamed, and of 17 to 64 rows where tiles would be modelled slower or need copies
+    // (bf16, 4096 -> 11264 -> 4096, streamed / tiles: 16 rows 64 / 73 us, 24 rows 81 / 73, 64 rows 132 / 79;
+    // 512 -> 2048 -> 512: 24 rows 10.9 / 14.2, 64 rows 16.8 / 14.4; 288 -> 256 -> 288: 64 rows 7.6 / 9.3)
     const Shape gs{M, 2L * F}, ds{M, E};
-    const TileChoice gc = choose<T>(&gs, 1, E, false), dc = choose<T>(&ds, 1, F, true);
-    slabs(D, dc.split, ws);
+    const TileChoice gc = choose<T>(&gs, 1, E, 1, false, (A.a ? 8 + sizeof(T) : sizeof(T)) / 2.0),
+                     dc = choose<T>(&ds, 1, F, 1, true, sizeof(T));
+    const bool few = M <= kFewRows && !forced_tile;
+    const bool stream_in = few && (M <= 16 || !direct_in(A) || few_rows_us<T>(M, F, E, 2) <= gc.us);
+    const bool stream_out = few && (M <= 16 || !Packer::direct(A.w_down, A.ld_down, F) || few_rows_us<T>(M, E, F, 1) <= dc.us);
+    Packer pk(ws);
+    Launch G{}, D{};
+    if (!stream_in) {
+      Operand x = pk.take(A.x, A.ld_x, M, E), gate, up;
+      take_pair(pk, A, gate, up);
+      G.count = 1;
+      G.act = A.activation;
+      Problem &g = G.p[0];
+      operands(g, x, gate);
+      g.b[1] = up.p;
+      g.M = M; g.N = F; g.K = E;
+      g.c = A.h; g.ldc = A.ld_h; g.pad = (int)A.ld_h;
+      g.bias0 = A.b_gate; g.bias1 = A.b_up;
+      g.out0 = A.a; g.out1 = A.b; g.ldaux = A.ld_h;
+    }
+    if (!stream_out) {
+      Operand down = pk.take(A.w_down, A.ld_down, E, F);
+      D.count = 1;
+      Problem &d = D.p[0];
+      operands(d, Operand{A.h, A.ld_h}, down);
+      d.M = M; d.N = E; d.K = F;
+      d.c = A.y; d.ldc = A.ld_y; d.bias0 = A.b_down;
+      slabs(D, dc.split, ws);
+    }
     if (!run) return hipSuccess;
     if ((err = pk.run(stream)) != hipSuccess) return err;
-    if ((err = run_tiles<T, kGateUp, kNT>(G, gc.size, stream)) != hipSuccess) return err;
+    if (stream_in) {
+      FewRows P{A.x, A.w_gate, A.w_up, A.ld_x, A.ld_gate, A.ld_up, M, F, E, A.activation, A.h, A.ld_h, (int)A.ld_h,
+                A.b_gate, A.b_up, A.a, A.b, A.ld_h};
+      err = few_rows<2>(P, stream);
+    } else {
+      err = run_tiles<T, kGateUp, kNT>(G, gc.size, stream);
+    }
+    if (err != hipSuccess) return err;
+    if (stream_out) {
+      FewRows P{A.h, A.w_down, A.w_down, A.ld_h, A.ld_down, A.ld_down, M, E, F, A.activation, A.y, A.ld_y, 0,
+                A.b_down, nullptr, nullptr, nullptr, 0};
+      return few_rows<1>(P, stream);
+    }
     if ((err = run_tiles<T, kPlain, kNT>(D, dc.size, stream)) != hipSuccess) return err;
     return fold(D, stream);
   }
@@ -497,7 +542,7 @@ template <typename T> struct Block {
     if (A.dx) take_pair(pk, A, gate, up);
     Operand da{}, db{};
     Launch G{}, X{}, W{};
-    TileChoice gc{64, 1}, xc{64, 1}, wc{64, 1};
+    TileChoice gc{}, xc{}, wc{};
     if (inner) {
       down = pk.take(A.w_down, A.ld_down, E, F);
       da = Operand{ws.take(A.ld_h * (long)M * (long)sizeof(T)), A.ld_h};
@@ -510,7 +555,7 @@ template <typename T> struct Block {
       g.c = (void *)da.p; g.c2 = (void *)db.p; g.ldc = A.ld_h; g.pad = (int)A.ld_h;
       g.aux0 = A.a; g.aux1 = A.b; g.ldaux = A.ld_h;
       const Shape s{M, F};
-      gc = choose<T>(&s, 1, E, false);
+      gc = choose<T>(&s, 1, E, 1, false, 8 + 2 * sizeof(T));
     }
     if (A.dx) {
       X.count = 1;
@@ -521,7 +566,7 @@ template <typename T> struct Block {
       p.M = M; p.N = E; p.K = F;
       p.c = A.dx; p.ldc = A.ld_dx;
       const Shape s{M, E};
-      xc = choose<T>(&s, 1, 2L * F, true);
+      xc = choose<T>(&s, 1, F, 2, true, sizeof(T));
       slabs(X, xc.split, ws);
     }
     Shape ws_shapes[3];
@@ -536,7 +581,7 @@ template <typename T> struct Block {
     if (A.dw_up) weight(db, x, F, E, A.dw_up);
     if (A.dw_down) weight(dy, Operand{A.h, A.ld_h}, E, F, A.dw_down);
     if (W.count) {
-      wc = choose<T>(ws_shapes, W.count, M, true);
+      wc = choose<T>(ws_shapes, W.count, M, 1, true, sizeof(T));
       slabs(W, wc.split, ws);
     }
     // bias gradients: column sums of da, db, dy in row chunks
@@ -552,9 +597,10 @@ template <typename T> struct Block {
     if (A.db_up) column(db.p, A.ld_h, F, A.db_up);
     if (A.db_down) column(A.dy, A.ld_dy, E, A.db_down);
     if (S.count) {
-      long chunks = (8L * kCUs + blocks - 1) / blocks;   // about eight workgroups per CU, at least 32 rows each
-      const long most = ((long)M + 31) / 32;
-      S.chunks = (int)(chunks < 1 ? 1 : (chunks > most ? most : chunks));
+      // about four workgroups per CU, at least 32 rows each, few enough for one thread to fold
+      long chunks = (4L * kCUs + blocks - 1) / blocks;
+      const long most = ((long)M + 31) / 32 < 48 ? ((long)M + 31) / 32 : 48;
+      S.chunks = (int)(chunks > most ? most : chunks);
       for (int i = 0; i < S.count; ++i) S.c[i].part = (float *)ws.take((long)S.chunks * S.c[i].cols * 4);
     }
     if (!run) return hipSuccess;
@@ -563,18 +609,17 @@ template <typename T> struct Block {
     if (S.count) {
       hipLaunchKernelGGL((column_sum_kernel<T>), dim3((unsigned)blocks, (unsigned)S.chunks), dim3(256), 0, stream, S);
       if ((err = hipGetLastError()) != hipSuccess) return err;
-      hipLaunchKernelGGL((column_sum_fold_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, S);
-      if ((err = hipGetLastError()) != hipSuccess) return err;
     }
     if (A.dx) {
       if ((err = run_tiles<T, kPlain, kNN>(X, xc.size, stream)) != hipSuccess) return err;
       if ((err = fold(X, stream)) != hipSuccess) return err;
     }
-    if (W.count) {
-      if ((err = run_tiles<T, kPlain, kTN>(W, wc.size, stream)) != hipSuccess) return err;
-      if ((err = fold(W, stream)) != hipSuccess) return err;
-    }
-    return hipSuccess;
+    if (W.count && (err = run_tiles<T, kPlain, kTN>(W, wc.size, stream)) != hipSuccess) return err;
+    // the weight gradients' slabs and the bias gradients' row chunks in one launch
+    Folds last{};
+    add_folds(last, W);
+    for (int i = 0; i < S.count; ++i) add_fold(last, S.c[i].part, S.c[i].cols, S.chunks, 1, S.c[i].cols, S.c[i].out, S.c[i].cols, nullptr);
+    return run_folds(last, stream);
   }
 };
 

@@ -18,8 +18,9 @@ bool valid(const butd_gated_ffn_args *a, bool backward) {
   if (!a || a->dtype < BUTD_FFN_F32 || a->dtype > BUTD_FFN_F16) return false;
   if (a->activation < BUTD_FFN_SILU || a->activation > BUTD_FFN_SIGMOID) return false;
   if (a->rows < 0 || a->rows > 0x7fffffffL || a->width < 1 || a->hidden < 1) return false;
-  // (a tile's last column index, and twice the hidden width, have to fit an int)
-  if (a->width > (1 << 28) || a->hidden > (1 << 28)) return false;
+  // (offsets inside a tile's 256 rows have to fit 31 bits)
+  constexpr long kMost = 1L << 20;
+  if (a->width > kMost || a->hidden > kMost) return false;
   if (a->ld_gate < a->width || a->ld_up < a->width || a->ld_down < a->hidden) return false;
   if (a->ld_h != butd_gated_ffn_ld_hidden(a->dtype, a->hidden)) return false;
   if (a->rows == 0) return true;
@@ -31,8 +32,8 @@ bool valid(const butd_gated_ffn_args *a, bool backward) {
   if (!a->x || a->ld_x < a->width || !a->w_gate || !a->w_up || !a->w_down) return false;
   if (!a->h || ((uintptr_t)a->h | (uintptr_t)a->a | (uintptr_t)a->b) & 15) return false;
   if ((a->a == nullptr) != (a->b == nullptr)) return false;
-  if (!backward) return a->y && a->ld_y >= a->width;
-  return a->a && a->dy && a->ld_dy >= a->width && (!a->dx || a->ld_dx >= a->width);
+  if (!backward) return a->y && a->ld_y >= a->width && a->ld_y <= kMost;
+  return a->a && a->dy && a->ld_dy >= a->width && (!a->dx || (a->ld_dx >= a->width && a->ld_dx <= kMost));
 }
 
 hipError_t dispatch(const butd_gated_ffn_args &a, ffn::Arena &ws, bool run, hipStream_t stream, bool backward) {

@@ -33,7 +33,7 @@ enum { BUTD_FFN_SILU = 0, BUTD_FFN_GELU = 1, BUTD_FFN_GELU_TANH = 2, BUTD_FFN_RE
 typedef struct {
   int dtype, activation;
   long rows;                        /* tokens, 0 .. 2^31 - 1 */
-  int width, hidden;                /* E, F >= 1 */
+  int width, hidden;                /* E, F: 1 .. 2^20 */
   const void *x;                    /* (rows, E) */
   const void *w_gate, *w_up;        /* (F, E) */
   const void *w_down;               /* (E, F) */
@@ -47,7 +47,7 @@ typedef struct {
   float *a, *b;
   long ld_h;
   void *y;                          /* (rows, E), forward */
-  long ld_y;
+  long ld_y;                        /* ld_y, ld_dx: up to 2^20 */
   /* backward: dy in; every other pointer may be NULL (that gradient is not computed).  Weight gradients are dense. */
   const void *dy;                   /* (rows, E) */
   long ld_dy;
