@@ -22,39 +22,56 @@ typedef butd_residual_norm_args Args;
 constexpr int N = 8;           // consecutive elements of a row in a thread: 16 bytes of a 16-bit tensor, two loads of a 32-bit one
 
 // ---- N consecutive elements of type T at any address, `left` of them existing --------------------------------------------
-template <typename T> __device__ inline void load(const T *p, int left, float *v) {
-  if (left >= N) {
+// WHOLE: the row's length is a multiple of N, a thread has all of its elements or none
+template <bool WHOLE, typename T> __device__ inline void load(const T *p, int left, float *v) {
+  if (WHOLE ? left > 0 : left >= N) {
     T e[N];
     __builtin_memcpy(e, p, N * sizeof(T));
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (float)e[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = i < left ? (float)p[i] : 0.f;
+    for (int i = 0; i < N; ++i) v[i] = !WHOLE && i < left ? (float)p[i] : 0.f;
   }
 }
-template <typename T> __device__ inline void store(T *p, int left, const float *v) {
-  if (left >= N) {
+template <bool WHOLE, typename T> __device__ inline void store(T *p, int left, const float *v) {
+  if (WHOLE ? left > 0 : left >= N) {
     T e[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) e[i] = (T)v[i];
     __builtin_memcpy(p, e, N * sizeof(T));
-  } else {
+  } else if (!WHOLE) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (i < left) p[i] = (T)v[i];
   }
 }
+// the same elements as they lie in memory, loaded now and widened later
+template <bool WHOLE, typename T> struct Raw {
+  T e[N];
+  __device__ inline void load(const T *p, int left) {
+    if (WHOLE ? left > 0 : left >= N) {
+      __builtin_memcpy(e, p, N * sizeof(T));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) e[i] = !WHOLE && i < left ? p[i] : (T)0.f;
+    }
+  }
+  __device__ inline void widen(float *v) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (float)e[i];
+  }
+};
 // parameters: the type of x or 32 bits; one that is not there is `value`.  Behind the row's end: zeros, which keeps the
 // elements there out of every sum without a test.
-template <typename T> __device__ inline void load_param(const void *p, bool f32, long at, int left, float value, float *v) {
+template <bool WHOLE, typename T> __device__ inline void load_param(const void *p, bool f32, long at, int left, float value, float *v) {
   if (!p) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = i < left ? value : 0.f;
+    for (int i = 0; i < N; ++i) v[i] = (WHOLE ? 0 : i) < left ? value : 0.f;
   } else if (f32) {
-    load<float>((const float *)p + at, left, v);
+    load<WHOLE, float>((const float *)p + at, left, v);
   } else {
-    load<T>((const T *)p + at, left, v);
+    load<WHOLE, T>((const T *)p + at, left, v);
   }
 }
 
@@ -104,7 +121,7 @@ template <int TPR> struct Group {
   static constexpr int kRows = kThreads / TPR;
 };
 
-template <typename T, typename R, int TPR>
+template <typename T, typename R, int TPR, bool WHOLE>
 __global__ __launch_bounds__(Group<TPR>::kThreads) void forward_kernel(const Args A) {
   __shared__ float sums[2][TPR / 64][1];
   __builtin_amdgcn_s_setprio(BUTD_MAIN_PRIO);
@@ -114,17 +131,17 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void forward_kernel(const Arg
   if (row >= A.rows) return;                             // (whole waves, or the whole workgroup)
   // everything the row needs is on its way before the first sum
   float x[N], r[N], w1[N], b1[N], g[N], w2[N], b2[N];
-  load<T>((const T *)A.x + at, left, x);
-  if (A.residual) load<R>((const R *)A.residual + at, left, r);
+  load<WHOLE, T>((const T *)A.x + at, left, x);
+  if (A.residual) load<WHOLE, R>((const R *)A.residual + at, left, r);
   const long gate_row = A.gate_kind == BUTD_GATE_ELEMENT ? row : A.gate_kind == BUTD_GATE_SAMPLE ? row / A.rows_per_sample : 0;
-  load_param<T>(A.gate, A.gate_dtype == BUTD_NORM_F32, gate_row * cols + c, left, 1.f, g);
+  load_param<WHOLE, T>(A.gate, A.gate_dtype == BUTD_NORM_F32, gate_row * cols + c, left, 1.f, g);
   if (A.post_kind) {
-    load_param<T>(A.post_weight, A.post_dtype == BUTD_NORM_F32, c, left, 1.f, w1);
-    load_param<T>(A.post_bias, A.post_dtype == BUTD_NORM_F32, c, left, 0.f, b1);
+    load_param<WHOLE, T>(A.post_weight, A.post_dtype == BUTD_NORM_F32, c, left, 1.f, w1);
+    load_param<WHOLE, T>(A.post_bias, A.post_dtype == BUTD_NORM_F32, c, left, 0.f, b1);
   }
   if (A.pre_kind) {
-    load_param<T>(A.pre_weight, A.pre_dtype == BUTD_NORM_F32, c, left, 1.f, w2);
-    load_param<T>(A.pre_bias, A.pre_dtype == BUTD_NORM_F32, c, left, 0.f, b2);
+    load_param<WHOLE, T>(A.pre_weight, A.pre_dtype == BUTD_NORM_F32, c, left, 1.f, w2);
+    load_param<WHOLE, T>(A.pre_bias, A.pre_dtype == BUTD_NORM_F32, c, left, 0.f, b2);
   }
   // v -> (v - mean) / deviation
   auto normalise = [&](float *v, int kind, float eps, float *stats) {
@@ -136,7 +153,7 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void forward_kernel(const Arg
       row_sum(s);
       mean = s[0] / (float)cols;
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = i < left ? v[i] - mean : 0.f;
+      for (int i = 0; i < N; ++i) v[i] = (WHOLE ? 0 : i) < left ? v[i] - mean : 0.f;
     }
     float s[1] = {0.f};
 #pragma unroll
@@ -160,12 +177,12 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void forward_kernel(const Arg
     x[i] *= g[i];
     if (A.residual) x[i] += A.residual_scale * r[i];
   }
-  if (A.stream) store<R>((R *)A.stream + at, left, x);
+  if (A.stream) store<WHOLE, R>((R *)A.stream + at, left, x);
   if (!A.pre_kind) return;
   normalise(x, A.pre_kind, A.pre_eps, A.stats ? A.stats + 2 * A.rows : nullptr);
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = x[i] * w2[i] + b2[i];
-  store<T>((T *)A.normed + at, left, x);
+  store<WHOLE, T>((T *)A.normed + at, left, x);
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------------
@@ -183,7 +200,7 @@ struct Plan {
 
 enum { kPostW = 0, kPostB, kPreW, kPreB };
 
-template <typename T, typename R, int TPR>
+template <typename T, typename R, int TPR, bool WHOLE>
 __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Args A, const Plan P) {
   constexpr int kRows = Group<TPR>::kRows;
   __shared__ float sums[2][TPR / 64][2];
@@ -200,9 +217,9 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
   const long segment = by_sample ? A.rows_per_sample : A.rows;
 
   float w1[N], b1[N], w2[N], g[N];
-  load_param<T>(post ? A.post_weight : nullptr, A.post_dtype == BUTD_NORM_F32, c, left, 1.f, w1);
-  load_param<T>(post ? A.post_bias : nullptr, A.post_dtype == BUTD_NORM_F32, c, left, 0.f, b1);
-  load_param<T>(pre ? A.pre_weight : nullptr, A.pre_dtype == BUTD_NORM_F32, c, left, 1.f, w2);
+  load_param<WHOLE, T>(post ? A.post_weight : nullptr, A.post_dtype == BUTD_NORM_F32, c, left, 1.f, w1);
+  load_param<WHOLE, T>(post ? A.post_bias : nullptr, A.post_dtype == BUTD_NORM_F32, c, left, 0.f, b1);
+  load_param<WHOLE, T>(pre ? A.pre_weight : nullptr, A.pre_dtype == BUTD_NORM_F32, c, left, 1.f, w2);
   float sum_w1[N], sum_b1[N], sum_w2[N], sum_b2[N], sum_g[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) sum_w1[i] = sum_b1[i] = sum_w2[i] = sum_b2[i] = sum_g[i] = 0.f;
@@ -222,40 +239,52 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
 #pragma unroll
           for (int s = 1; s < kRows; ++s) v[i] += joined[s][i * 64 + th];
         }
-        store<float>(dst + c, left, v);
+        store<WHOLE, float>(dst + c, left, v);
       }
     } else {
-      store<float>(dst + c, left, sum);
+      store<WHOLE, float>(dst + c, left, sum);
     }
   };
 
+  // a row's tensors and statistics, loaded while the row before is worked on
+  struct Ahead {
+    Raw<WHOLE, T> x, u;
+    Raw<WHOLE, R> n, d;
+    float stats[4];
+  };
+  auto fetch = [&](Ahead &h, long row) {
+    const long at = row * cols + c;
+    h.x.load((const T *)A.x + at, left);
+    h.n.load((const R *)A.residual + at, pre && A.residual ? left : 0);
+    h.u.load((const T *)A.d_normed + at, pre ? left : 0);
+    h.d.load((const R *)A.d_stream + at, A.d_stream ? left : 0);
+    h.stats[0] = post ? A.stats[row] : 0.f;
+    h.stats[1] = post ? A.stats[A.rows + row] : 1.f;
+    h.stats[2] = pre ? A.stats[2 * A.rows + row] : 0.f;
+    h.stats[3] = pre ? A.stats[3 * A.rows + row] : 1.f;
+  };
   for (long s0 = first; s0 < last;) {
     const long s1 = by_sample ? min(last, (s0 / segment + 1) * segment) : last;
-    if (!by_element) load_param<T>(A.gate, A.gate_dtype == BUTD_NORM_F32, (by_sample ? s0 / segment : 0) * cols + c, left, 1.f, g);
+    if (!by_element) load_param<WHOLE, T>(A.gate, A.gate_dtype == BUTD_NORM_F32, (by_sample ? s0 / segment : 0) * cols + c, left, 1.f, g);
+    Ahead ahead;
+    if (s0 + sub < s1) fetch(ahead, s0 + sub);
     for (long row = s0 + sub; row < s1; row += kRows) {  // (several rows: each is one wave's, nothing below waits for another wave)
       const long at = row * cols + c;
       float x[N], n[N], u[N], d[N];
-      load<T>((const T *)A.x + at, left, x);
-      if (by_element) load_param<T>(A.gate, A.gate_dtype == BUTD_NORM_F32, at, left, 1.f, g);
-      if (pre) {
-        if (A.residual) load<R>((const R *)A.residual + at, left, n);
-        load<T>((const T *)A.d_normed + at, left, u);
-      }
-      if (A.d_stream) load<R>((const R *)A.d_stream + at, left, d);
-      else
-#pragma unroll
-        for (int i = 0; i < N; ++i) d[i] = 0.f;
-      float rstd1 = 1.f;
+      ahead.x.widen(x);
+      ahead.n.widen(n);
+      ahead.u.widen(u);
+      ahead.d.widen(d);
+      const float mean1 = ahead.stats[0], rstd1 = ahead.stats[1], mean2 = ahead.stats[2], rstd2 = ahead.stats[3];
+      if (by_element) load_param<WHOLE, T>(A.gate, A.gate_dtype == BUTD_NORM_F32, at, left, 1.f, g);
+      if (row + kRows < s1) fetch(ahead, row + kRows);   // on its way while this row is worked on
       if (post) {
-        const float mean1 = A.stats[row];
-        rstd1 = A.stats[A.rows + row];
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = (x[i] - mean1) * rstd1;
       }
       float s[2];
       if (pre) {
         // the stream again, normalised: n;  d += rstd2 (u - mean(u) - n mean(u n)),  u = d_normed * weight
-        const float mean2 = A.stats[2 * A.rows + row], rstd2 = A.stats[3 * A.rows + row];
         s[0] = s[1] = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -277,7 +306,7 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
         float v[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = A.residual_scale * d[i];
-        store<R>((R *)A.d_residual + at, left, v);
+        store<WHOLE, R>((R *)A.d_residual + at, left, v);
       }
       s[0] = s[1] = 0.f;
 #pragma unroll
@@ -292,8 +321,8 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
         s[1] += d[i] * x[i];
       }
       if (by_element && A.d_gate) {
-        if (A.gate_dtype == BUTD_NORM_F32) store<float>((float *)A.d_gate + at, left, u);
-        else store<T>((T *)A.d_gate + at, left, u);
+        if (A.gate_dtype == BUTD_NORM_F32) store<WHOLE, float>((float *)A.d_gate + at, left, u);
+        else store<WHOLE, T>((T *)A.d_gate + at, left, u);
       }
       if (post) {
         row_sum(s);
@@ -301,7 +330,7 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
 #pragma unroll
         for (int i = 0; i < N; ++i) d[i] = rstd1 * (d[i] - m0 - x[i] * m1);
       }
-      if (A.d_x) store<T>((T *)A.d_x + at, left, d);
+      if (A.d_x) store<WHOLE, T>((T *)A.d_x + at, left, d);
     }
     if (by_sample && P.gate_part) {
       flush(sum_g, P.gate_part + (P.run == segment ? (long)blockIdx.x : s0 / segment) * cols);
@@ -398,7 +427,8 @@ template <typename T, typename R> struct Forward {
   hipStream_t stream;
   template <int TPR> hipError_t operator()() {
     const long blocks = (A.rows + Group<TPR>::kRows - 1) / Group<TPR>::kRows;
-    hipLaunchKernelGGL((forward_kernel<T, R, TPR>), dim3((unsigned)blocks), dim3(Group<TPR>::kThreads), 0, stream, A);
+    auto *kernel = A.cols % N ? &forward_kernel<T, R, TPR, false> : &forward_kernel<T, R, TPR, true>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(Group<TPR>::kThreads), 0, stream, A);
     return hipGetLastError();
   }
 };
@@ -447,7 +477,8 @@ template <typename T, typename R> struct Backward {
   const Plan &P;
   hipStream_t stream;
   template <int TPR> hipError_t operator()() {
-    hipLaunchKernelGGL((backward_kernel<T, R, TPR>), dim3((unsigned)P.blocks), dim3(Group<TPR>::kThreads), 0, stream, A, P);
+    auto *kernel = A.cols % N ? &backward_kernel<T, R, TPR, false> : &backward_kernel<T, R, TPR, true>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)P.blocks), dim3(Group<TPR>::kThreads), 0, stream, A, P);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     Folds L;
