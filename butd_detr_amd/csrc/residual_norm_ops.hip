@@ -18,6 +18,7 @@
 namespace {
 
 typedef butd_residual_norm_args Args;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int N = 8;           // consecutive elements of a row in a thread: 16 bytes of a 16-bit tensor, two loads of a 32-bit one
 
@@ -122,7 +123,7 @@ template <int TPR> struct Group {
 };
 
 template <typename T, typename R, int TPR, bool WHOLE>
-__global__ __launch_bounds__(Group<TPR>::kThreads) void forward_kernel(const Args A) {
+__global__ __launch_bounds__(Group<TPR>::kThreads, TPR == 1024 ? 8 : 1) void forward_kernel(const Args A) {
   __shared__ float sums[2][TPR / 64][1];
   __builtin_amdgcn_s_setprio(BUTD_MAIN_PRIO);
   RowSum<TPR, 1> row_sum{sums};
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void forward_kernel(const Arg
   const long row = (long)blockIdx.x * Group<TPR>::kRows + sub, at = row * cols + c;
   if (row >= A.rows) return;                             // (whole waves, or the whole workgroup)
   // everything the row needs is on its way before the first sum
-  float x[N], r[N], w1[N], b1[N], g[N], w2[N], b2[N];
+  float x[N], r[N], w1[N], b1[N], g[N];
   load<WHOLE, T>((const T *)A.x + at, left, x);
   if (A.residual) load<WHOLE, R>((const R *)A.residual + at, left, r);
   const long gate_row = A.gate_kind == BUTD_GATE_ELEMENT ? row : A.gate_kind == BUTD_GATE_SAMPLE ? row / A.rows_per_sample : 0;
@@ -138,10 +139,6 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void forward_kernel(const Arg
   if (A.post_kind) {
     load_param<WHOLE, T>(A.post_weight, A.post_dtype == BUTD_NORM_F32, c, left, 1.f, w1);
     load_param<WHOLE, T>(A.post_bias, A.post_dtype == BUTD_NORM_F32, c, left, 0.f, b1);
-  }
-  if (A.pre_kind) {
-    load_param<WHOLE, T>(A.pre_weight, A.pre_dtype == BUTD_NORM_F32, c, left, 1.f, w2);
-    load_param<WHOLE, T>(A.pre_bias, A.pre_dtype == BUTD_NORM_F32, c, left, 0.f, b2);
   }
   // v -> (v - mean) / deviation
   auto normalise = [&](float *v, int kind, float eps, float *stats) {
@@ -179,6 +176,9 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void forward_kernel(const Arg
   }
   if (A.stream) store<WHOLE, R>((R *)A.stream + at, left, x);
   if (!A.pre_kind) return;
+  float w2[N], b2[N];                                    // on their way during the second norm's sums
+  load_param<WHOLE, T>(A.pre_weight, A.pre_dtype == BUTD_NORM_F32, c, left, 1.f, w2);
+  load_param<WHOLE, T>(A.pre_bias, A.pre_dtype == BUTD_NORM_F32, c, left, 0.f, b2);
   normalise(x, A.pre_kind, A.pre_eps, A.stats ? A.stats + 2 * A.rows : nullptr);
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = x[i] * w2[i] + b2[i];
@@ -220,16 +220,46 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
   load_param<WHOLE, T>(post ? A.post_weight : nullptr, A.post_dtype == BUTD_NORM_F32, c, left, 1.f, w1);
   load_param<WHOLE, T>(post ? A.post_bias : nullptr, A.post_dtype == BUTD_NORM_F32, c, left, 0.f, b1);
   load_param<WHOLE, T>(pre ? A.pre_weight : nullptr, A.pre_dtype == BUTD_NORM_F32, c, left, 1.f, w2);
-  float sum_w1[N], sum_b1[N], sum_w2[N], sum_b2[N], sum_g[N];
+  // column sums: a thread's own, in registers; those of a row on 1024 threads (128 registers each) in LDS
+  constexpr bool kInLds = TPR == 1024;
+  constexpr int kSums = kInLds ? 1 : 4;
+  __shared__ f32x4 shared_sums[kInLds ? 4 : 1][2][kInLds ? TPR : 1];
+  float sum[kSums][N], sum_g[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) sum_w1[i] = sum_b1[i] = sum_w2[i] = sum_b2[i] = sum_g[i] = 0.f;
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) sum[k][i] = 0.f;
+    sum_g[i] = 0.f;
+  }
+  if constexpr (kInLds) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) shared_sums[k][0][th] = shared_sums[k][1][th] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  auto add = [&](int k, const float *v) {
+    if constexpr (kInLds) {
+      shared_sums[k][0][th] += f32x4{v[0], v[1], v[2], v[3]};
+      shared_sums[k][1][th] += f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum[k][i] += v[i];
+    }
+  };
+  auto total = [&](int k, float *v) {
+    if constexpr (kInLds) {
+      __builtin_memcpy(v, &shared_sums[k][0][th], 16);
+      __builtin_memcpy(v + 4, &shared_sums[k][1][th], 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = sum[k][i];
+    }
+  };
 
   // column sums of the workgroup: over its rows side by side through LDS, then out
-  auto flush = [&](float *sum, float *dst) {
+  auto flush = [&](const float *own, float *dst) {
     if constexpr (kRows > 1) {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < N; ++i) joined[sub][i * 64 + th] = sum[i];
+      for (int i = 0; i < N; ++i) joined[sub][i * 64 + th] = own[i];
       __syncthreads();
       if (sub == 0) {
         float v[N];
@@ -242,7 +272,7 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
         store<WHOLE, float>(dst + c, left, v);
       }
     } else {
-      store<WHOLE, float>(dst + c, left, sum);
+      store<WHOLE, float>(dst + c, left, own);
     }
   };
 
@@ -285,14 +315,19 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
       float s[2];
       if (pre) {
         // the stream again, normalised: n;  d += rstd2 (u - mean(u) - n mean(u n)),  u = d_normed * weight
-        s[0] = s[1] = 0.f;
+        float v[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           float t = g[i] * (x[i] * w1[i] + b1[i]);
           if (A.residual) t += A.residual_scale * n[i];
           n[i] = (t - mean2) * rstd2;
-          sum_w2[i] += u[i] * n[i];
-          sum_b2[i] += u[i];
+          v[i] = u[i] * n[i];
+        }
+        add(kPreW, v);
+        add(kPreB, u);
+        s[0] = s[1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
           u[i] *= w2[i];
           s[0] += u[i];
           s[1] += u[i] * n[i];
@@ -308,23 +343,27 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
         for (int i = 0; i < N; ++i) v[i] = A.residual_scale * d[i];
         store<WHOLE, R>((R *)A.d_residual + at, left, v);
       }
-      s[0] = s[1] = 0.f;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         u[i] = d[i] * (x[i] * w1[i] + b1[i]);            // the gate's gradient
         sum_g[i] += u[i];
-        const float dt = d[i] * g[i];
-        sum_w1[i] += dt * x[i];
-        sum_b1[i] += dt;
-        d[i] = dt * w1[i];
-        s[0] += d[i];
-        s[1] += d[i] * x[i];
+        d[i] *= g[i];
+        n[i] = d[i] * x[i];
       }
       if (by_element && A.d_gate) {
         if (A.gate_dtype == BUTD_NORM_F32) store<WHOLE, float>((float *)A.d_gate + at, left, u);
         else store<WHOLE, T>((T *)A.d_gate + at, left, u);
       }
       if (post) {
+        add(kPostW, n);
+        add(kPostB, d);
+        s[0] = s[1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          s[0] += d[i] * w1[i];
+          s[1] += n[i] * w1[i];
+          d[i] *= w1[i];
+        }
         row_sum(s);
         const float m0 = A.post_kind == BUTD_NORM_LAYER ? s[0] * inv_cols : 0.f, m1 = s[1] * inv_cols;
 #pragma unroll
@@ -342,10 +381,14 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
   if (A.gate_kind == BUTD_GATE_CHANNEL && P.gate_part) flush(sum_g, P.gate_part + (long)blockIdx.x * cols);
   if (P.part) {
     float *dst = P.part + (long)blockIdx.x * 4 * cols;
-    if (A.d_post_weight) flush(sum_w1, dst + kPostW * (long)cols);
-    if (A.d_post_bias) flush(sum_b1, dst + kPostB * (long)cols);
-    if (A.d_pre_weight) flush(sum_w2, dst + kPreW * (long)cols);
-    if (A.d_pre_bias) flush(sum_b2, dst + kPreB * (long)cols);
+    float v[N];
+    void *const wanted[4] = {A.d_post_weight, A.d_post_bias, A.d_pre_weight, A.d_pre_bias};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (wanted[k]) {
+        total(k, v);
+        flush(v, dst + k * (long)cols);
+      }
   }
 }
 
