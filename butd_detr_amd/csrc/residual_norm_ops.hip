@@ -4,7 +4,7 @@
 // gradients and writes two.  A row's values stay in registers from the load to the last use (both norms' statistics are
 // sums over registers, the deviations taken around the mean, not as a difference of squares), so each tensor is touched
 // once.  Rows of up to 512 elements belong to ONE wave and are reduced inside it; wider rows to a workgroup.  Rows of any
-// width and address: 16 bytes a lane wherever the row still has them, elements at its end.
+// width and address, 16 bytes a lane.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -22,57 +22,73 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int N = 8;           // consecutive elements of a row in a thread: 16 bytes of a 16-bit tensor, two loads of a 32-bit one
 
+// How threads share a row out, N elements each, the first `left` of them existing.
+//   kWhole     a length that is a multiple of N: all of a thread's elements exist, or none
+//   kOverlap   any other length above N: the last unit is moved back to end with the row, so every access is a whole unit.
+//              The first `twice` elements of it are its neighbour's too: both threads compute and write the same values, and
+//              the row's sums take the neighbour's.  (1537 fp16 columns, 3003 rows: backward 24 us; 35 with the last
+//              unit element by element, whose eight predicates for every tensor spill scalar registers.)
+//   kElements  rows shorter than N
+enum Mode { kWhole, kOverlap, kElements };
+
 // ---- N consecutive elements of type T at any address, `left` of them existing --------------------------------------------
-// WHOLE: the row's length is a multiple of N, a thread has all of its elements or none
-template <bool WHOLE, typename T> __device__ inline void load(const T *p, int left, float *v) {
-  if (WHOLE ? left > 0 : left >= N) {
+template <Mode MODE, typename T> __device__ inline void load(const T *p, int left, float *v) {
+  if (MODE != kElements ? left > 0 : left >= N) {
     T e[N];
     __builtin_memcpy(e, p, N * sizeof(T));
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (float)e[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = !WHOLE && i < left ? (float)p[i] : 0.f;
+    for (int i = 0; i < N; ++i) v[i] = MODE == kElements && i < left ? (float)p[i] : 0.f;
   }
 }
-template <bool WHOLE, typename T> __device__ inline void store(T *p, int left, const float *v) {
-  if (WHOLE ? left > 0 : left >= N) {
+template <Mode MODE, typename T> __device__ inline void store(T *p, int left, const float *v) {
+  if (MODE != kElements ? left > 0 : left >= N) {
     T e[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) e[i] = (T)v[i];
     __builtin_memcpy(p, e, N * sizeof(T));
-  } else if (!WHOLE) {
+  } else if (MODE == kElements) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (i < left) p[i] = (T)v[i];
   }
 }
-// the same elements as they lie in memory, loaded now and widened later
-template <bool WHOLE, typename T> struct Raw {
-  T e[N];
+// the same elements as they lie in memory, loaded now and widened later.  (Held in 32-bit words: 16-bit elements that are
+// loaded on one side of a branch and zero on the other are packed there, which waits for the load.)
+template <Mode MODE, typename T> struct Raw {
+  static constexpr int kWords = N * sizeof(T) / 4;
+  uint32_t words[kWords];
   __device__ inline void load(const T *p, int left) {
-    if (WHOLE ? left > 0 : left >= N) {
-      __builtin_memcpy(e, p, N * sizeof(T));
-    } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) e[i] = !WHOLE && i < left ? p[i] : (T)0.f;
+    for (int i = 0; i < kWords; ++i) words[i] = 0;
+    if (MODE != kElements ? left > 0 : left >= N) {
+      __builtin_memcpy(words, p, sizeof(words));
+    } else if (MODE == kElements) {
+      T e[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) e[i] = i < left ? p[i] : (T)0.f;
+      __builtin_memcpy(words, e, sizeof(words));
     }
   }
   __device__ inline void widen(float *v) const {
+    T e[N];
+    __builtin_memcpy(e, words, sizeof(words));
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (float)e[i];
   }
 };
 // parameters: the type of x or 32 bits; one that is not there is `value`.  Behind the row's end: zeros, which keeps the
 // elements there out of every sum without a test.
-template <bool WHOLE, typename T> __device__ inline void load_param(const void *p, bool f32, long at, int left, float value, float *v) {
+template <Mode MODE, typename T> __device__ inline void load_param(const void *p, bool f32, long at, int left, float value, float *v) {
   if (!p) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = (WHOLE ? 0 : i) < left ? value : 0.f;
+    for (int i = 0; i < N; ++i) v[i] = (MODE != kElements ? 0 : i) < left ? value : 0.f;
   } else if (f32) {
-    load<WHOLE, float>((const float *)p + at, left, v);
+    load<MODE, float>((const float *)p + at, left, v);
   } else {
-    load<WHOLE, T>((const T *)p + at, left, v);
+    load<MODE, T>((const T *)p + at, left, v);
   }
 }
 
@@ -122,23 +138,25 @@ template <int TPR> struct Group {
   static constexpr int kRows = kThreads / TPR;
 };
 
-template <typename T, typename R, int TPR, bool WHOLE>
+template <typename T, typename R, int TPR, Mode MODE>
 __global__ __launch_bounds__(Group<TPR>::kThreads, TPR == 1024 ? 8 : 1) void forward_kernel(const Args A) {
   __shared__ float sums[2][TPR / 64][1];
   __builtin_amdgcn_s_setprio(BUTD_MAIN_PRIO);
   RowSum<TPR, 1> row_sum{sums};
-  const int sub = threadIdx.x / TPR, th = threadIdx.x % TPR, cols = A.cols, c = th * N, left = cols - c;
+  const int sub = threadIdx.x / TPR, th = threadIdx.x % TPR, cols = A.cols;
+  const int twice = MODE == kOverlap && th * N < cols ? max(th * N + N - cols, 0) : 0;
+  const int c = th * N - twice, left = cols - c;
   const long row = (long)blockIdx.x * Group<TPR>::kRows + sub, at = row * cols + c;
   if (row >= A.rows) return;                             // (whole waves, or the whole workgroup)
   // everything the row needs is on its way before the first sum
   float x[N], r[N], w1[N], b1[N], g[N];
-  load<WHOLE, T>((const T *)A.x + at, left, x);
-  if (A.residual) load<WHOLE, R>((const R *)A.residual + at, left, r);
+  load<MODE, T>((const T *)A.x + at, left, x);
+  if (A.residual) load<MODE, R>((const R *)A.residual + at, left, r);
   const long gate_row = A.gate_kind == BUTD_GATE_ELEMENT ? row : A.gate_kind == BUTD_GATE_SAMPLE ? row / A.rows_per_sample : 0;
-  load_param<WHOLE, T>(A.gate, A.gate_dtype == BUTD_NORM_F32, gate_row * cols + c, left, 1.f, g);
+  load_param<MODE, T>(A.gate, A.gate_dtype == BUTD_NORM_F32, gate_row * cols + c, left, 1.f, g);
   if (A.post_kind) {
-    load_param<WHOLE, T>(A.post_weight, A.post_dtype == BUTD_NORM_F32, c, left, 1.f, w1);
-    load_param<WHOLE, T>(A.post_bias, A.post_dtype == BUTD_NORM_F32, c, left, 0.f, b1);
+    load_param<MODE, T>(A.post_weight, A.post_dtype == BUTD_NORM_F32, c, left, 1.f, w1);
+    load_param<MODE, T>(A.post_bias, A.post_dtype == BUTD_NORM_F32, c, left, 0.f, b1);
   }
   // v -> (v - mean) / deviation
   auto normalise = [&](float *v, int kind, float eps, float *stats) {
@@ -146,15 +164,15 @@ __global__ __launch_bounds__(Group<TPR>::kThreads, TPR == 1024 ? 8 : 1) void for
     if (kind == BUTD_NORM_LAYER) {
       float s[1] = {0.f};
 #pragma unroll
-      for (int i = 0; i < N; ++i) s[0] += v[i];
+      for (int i = 0; i < N; ++i) s[0] += i >= twice ? v[i] : 0.f;
       row_sum(s);
       mean = s[0] / (float)cols;
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = (WHOLE ? 0 : i) < left ? v[i] - mean : 0.f;
+      for (int i = 0; i < N; ++i) v[i] = (MODE != kElements ? 0 : i) < left ? v[i] - mean : 0.f;
     }
     float s[1] = {0.f};
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[0] += v[i] * v[i];
+    for (int i = 0; i < N; ++i) s[0] += i >= twice ? v[i] * v[i] : 0.f;
     row_sum(s);
     const float rstd = 1.f / sqrtf(s[0] / (float)cols + eps);
 #pragma unroll
@@ -174,15 +192,15 @@ __global__ __launch_bounds__(Group<TPR>::kThreads, TPR == 1024 ? 8 : 1) void for
     x[i] *= g[i];
     if (A.residual) x[i] += A.residual_scale * r[i];
   }
-  if (A.stream) store<WHOLE, R>((R *)A.stream + at, left, x);
+  if (A.stream) store<MODE, R>((R *)A.stream + at, left, x);
   if (!A.pre_kind) return;
   float w2[N], b2[N];                                    // on their way during the second norm's sums
-  load_param<WHOLE, T>(A.pre_weight, A.pre_dtype == BUTD_NORM_F32, c, left, 1.f, w2);
-  load_param<WHOLE, T>(A.pre_bias, A.pre_dtype == BUTD_NORM_F32, c, left, 0.f, b2);
+  load_param<MODE, T>(A.pre_weight, A.pre_dtype == BUTD_NORM_F32, c, left, 1.f, w2);
+  load_param<MODE, T>(A.pre_bias, A.pre_dtype == BUTD_NORM_F32, c, left, 0.f, b2);
   normalise(x, A.pre_kind, A.pre_eps, A.stats ? A.stats + 2 * A.rows : nullptr);
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = x[i] * w2[i] + b2[i];
-  store<WHOLE, T>((T *)A.normed + at, left, x);
+  store<MODE, T>((T *)A.normed + at, left, x);
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------------
@@ -200,14 +218,16 @@ struct Plan {
 
 enum { kPostW = 0, kPostB, kPreW, kPreB };
 
-template <typename T, typename R, int TPR, bool WHOLE>
+template <typename T, typename R, int TPR, Mode MODE>
 __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Args A, const Plan P) {
   constexpr int kRows = Group<TPR>::kRows;
   __shared__ float sums[2][TPR / 64][2];
   __shared__ float joined[kRows > 1 ? kRows : 1][kRows > 1 ? 64 * N : 1];
   __builtin_amdgcn_s_setprio(BUTD_MAIN_PRIO);
   RowSum<TPR, 2> row_sum{sums};
-  const int sub = threadIdx.x / TPR, th = threadIdx.x % TPR, cols = A.cols, c = th * N, left = cols - c;
+  const int sub = threadIdx.x / TPR, th = threadIdx.x % TPR, cols = A.cols;
+  const int twice = MODE == kOverlap && th * N < cols ? max(th * N + N - cols, 0) : 0;
+  const int c = th * N - twice, left = cols - c;
   const float inv_cols = 1.f / (float)cols;
   const long run = blockIdx.x / P.share, piece = blockIdx.x - run * P.share;
   const long first = run * P.run + piece * P.per, last = min(first + P.per, min((run + 1) * P.run, A.rows));
@@ -217,9 +237,9 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
   const long segment = by_sample ? A.rows_per_sample : A.rows;
 
   float w1[N], b1[N], w2[N], g[N];
-  load_param<WHOLE, T>(post ? A.post_weight : nullptr, A.post_dtype == BUTD_NORM_F32, c, left, 1.f, w1);
-  load_param<WHOLE, T>(post ? A.post_bias : nullptr, A.post_dtype == BUTD_NORM_F32, c, left, 0.f, b1);
-  load_param<WHOLE, T>(pre ? A.pre_weight : nullptr, A.pre_dtype == BUTD_NORM_F32, c, left, 1.f, w2);
+  load_param<MODE, T>(post ? A.post_weight : nullptr, A.post_dtype == BUTD_NORM_F32, c, left, 1.f, w1);
+  load_param<MODE, T>(post ? A.post_bias : nullptr, A.post_dtype == BUTD_NORM_F32, c, left, 0.f, b1);
+  load_param<MODE, T>(pre ? A.pre_weight : nullptr, A.pre_dtype == BUTD_NORM_F32, c, left, 1.f, w2);
   // column sums: a thread's own, in registers; those of a row on 1024 threads (128 registers each) in LDS
   constexpr bool kInLds = TPR == 1024;
   constexpr int kSums = kInLds ? 1 : 4;
@@ -269,17 +289,18 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
 #pragma unroll
           for (int s = 1; s < kRows; ++s) v[i] += joined[s][i * 64 + th];
         }
-        store<WHOLE, float>(dst + c, left, v);
+        store<MODE, float>(dst + c, left, v);
       }
     } else {
-      store<WHOLE, float>(dst + c, left, own);
+      store<MODE, float>(dst + c, left, own);
     }
   };
 
-  // a row's tensors and statistics, loaded while the row before is worked on
+  // a row's tensors and statistics, loaded while the row before is worked on (not with 128 registers a thread)
+  constexpr bool kAhead = TPR < 1024;
   struct Ahead {
-    Raw<WHOLE, T> x, u;
-    Raw<WHOLE, R> n, d;
+    Raw<MODE, T> x, u;
+    Raw<MODE, R> n, d;
     float stats[4];
   };
   auto fetch = [&](Ahead &h, long row) {
@@ -295,19 +316,20 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
   };
   for (long s0 = first; s0 < last;) {
     const long s1 = by_sample ? min(last, (s0 / segment + 1) * segment) : last;
-    if (!by_element) load_param<WHOLE, T>(A.gate, A.gate_dtype == BUTD_NORM_F32, (by_sample ? s0 / segment : 0) * cols + c, left, 1.f, g);
+    if (!by_element) load_param<MODE, T>(A.gate, A.gate_dtype == BUTD_NORM_F32, (by_sample ? s0 / segment : 0) * cols + c, left, 1.f, g);
     Ahead ahead;
-    if (s0 + sub < s1) fetch(ahead, s0 + sub);
+    if (kAhead && s0 + sub < s1) fetch(ahead, s0 + sub);
     for (long row = s0 + sub; row < s1; row += kRows) {  // (several rows: each is one wave's, nothing below waits for another wave)
       const long at = row * cols + c;
       float x[N], n[N], u[N], d[N];
+      if (!kAhead) fetch(ahead, row);
       ahead.x.widen(x);
       ahead.n.widen(n);
       ahead.u.widen(u);
       ahead.d.widen(d);
       const float mean1 = ahead.stats[0], rstd1 = ahead.stats[1], mean2 = ahead.stats[2], rstd2 = ahead.stats[3];
-      if (by_element) load_param<WHOLE, T>(A.gate, A.gate_dtype == BUTD_NORM_F32, at, left, 1.f, g);
-      if (row + kRows < s1) fetch(ahead, row + kRows);   // on its way while this row is worked on
+      if (by_element) load_param<MODE, T>(A.gate, A.gate_dtype == BUTD_NORM_F32, at, left, 1.f, g);
+      if (kAhead && row + kRows < s1) fetch(ahead, row + kRows);   // on its way while this row is worked on
       if (post) {
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = (x[i] - mean1) * rstd1;
@@ -329,8 +351,8 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           u[i] *= w2[i];
-          s[0] += u[i];
-          s[1] += u[i] * n[i];
+          s[0] += i >= twice ? u[i] : 0.f;
+          s[1] += i >= twice ? u[i] * n[i] : 0.f;
         }
         row_sum(s);
         const float m0 = A.pre_kind == BUTD_NORM_LAYER ? s[0] * inv_cols : 0.f, m1 = s[1] * inv_cols;
@@ -341,7 +363,7 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
         float v[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = A.residual_scale * d[i];
-        store<WHOLE, R>((R *)A.d_residual + at, left, v);
+        store<MODE, R>((R *)A.d_residual + at, left, v);
       }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -351,8 +373,8 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
         n[i] = d[i] * x[i];
       }
       if (by_element && A.d_gate) {
-        if (A.gate_dtype == BUTD_NORM_F32) store<WHOLE, float>((float *)A.d_gate + at, left, u);
-        else store<WHOLE, T>((T *)A.d_gate + at, left, u);
+        if (A.gate_dtype == BUTD_NORM_F32) store<MODE, float>((float *)A.d_gate + at, left, u);
+        else store<MODE, T>((T *)A.d_gate + at, left, u);
       }
       if (post) {
         add(kPostW, n);
@@ -360,8 +382,8 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
         s[0] = s[1] = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          s[0] += d[i] * w1[i];
-          s[1] += n[i] * w1[i];
+          s[0] += i >= twice ? d[i] * w1[i] : 0.f;
+          s[1] += i >= twice ? n[i] * w1[i] : 0.f;
           d[i] *= w1[i];
         }
         row_sum(s);
@@ -369,7 +391,7 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
 #pragma unroll
         for (int i = 0; i < N; ++i) d[i] = rstd1 * (d[i] - m0 - x[i] * m1);
       }
-      if (A.d_x) store<WHOLE, T>((T *)A.d_x + at, left, d);
+      if (A.d_x) store<MODE, T>((T *)A.d_x + at, left, d);
     }
     if (by_sample && P.gate_part) {
       flush(sum_g, P.gate_part + (P.run == segment ? (long)blockIdx.x : s0 / segment) * cols);
@@ -470,17 +492,22 @@ template <typename T, typename R> struct Forward {
   hipStream_t stream;
   template <int TPR> hipError_t operator()() {
     const long blocks = (A.rows + Group<TPR>::kRows - 1) / Group<TPR>::kRows;
-    auto *kernel = A.cols % N ? &forward_kernel<T, R, TPR, false> : &forward_kernel<T, R, TPR, true>;
+    auto *kernel = A.cols % N == 0 ? &forward_kernel<T, R, TPR, kWhole> : &forward_kernel<T, R, TPR, kOverlap>;
+    if constexpr (TPR == 64)
+      if (A.cols < N) kernel = &forward_kernel<T, R, TPR, kElements>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(Group<TPR>::kThreads), 0, stream, A);
     return hipGetLastError();
   }
 };
 
-// the rows' shares: about `target` workgroups, whole samples each where the gate is one of the sample's
+// the rows' shares: about `target` workgroups, whole samples each where the gate is one of the sample's.  As many as run at
+// once, two waves a SIMD of the 180 to 220 registers: each workgroup more costs five partial rows, written and read again
+// (16384 rows of 4096 with both norms: 256 workgroups 237 + 4 us for the sums, 512 247 + 8, 768 251 + 12)
 Plan plan_of(const Args &A, char *ws, long *bytes) {
   Plan P{};
   const bool wave_rows = A.cols <= 64 * N;
-  const long step = wave_rows ? 4 : 1, target = wave_rows ? 1024 : 768;
+  const int threads = A.cols <= 64 * N ? 256 : A.cols <= 128 * N ? 128 : A.cols <= 256 * N ? 256 : 512;
+  const long step = wave_rows ? 4 : 1, target = 256 * (512 / threads);
   long per = (A.rows + target - 1) / target;
   per = (per + step - 1) / step * step;
   const long least = wave_rows ? 8 : 2;
@@ -520,7 +547,9 @@ template <typename T, typename R> struct Backward {
   const Plan &P;
   hipStream_t stream;
   template <int TPR> hipError_t operator()() {
-    auto *kernel = A.cols % N ? &backward_kernel<T, R, TPR, false> : &backward_kernel<T, R, TPR, true>;
+    auto *kernel = A.cols % N == 0 ? &backward_kernel<T, R, TPR, kWhole> : &backward_kernel<T, R, TPR, kOverlap>;
+    if constexpr (TPR == 64)
+      if (A.cols < N) kernel = &backward_kernel<T, R, TPR, kElements>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)P.blocks), dim3(Group<TPR>::kThreads), 0, stream, A, P);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
