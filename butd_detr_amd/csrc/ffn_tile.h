@@ -133,6 +133,8 @@ struct Problem {
   int tiles_m, tiles_n, first, steps, per_slice;
   uint32_t group_magic;
 };
+// rows of a slab are whole vectors
+__host__ __device__ inline int slab_ld(int n) { return (n + 3) & ~3; }
 constexpr int kMaxProblems = 3;
 struct Launch {
   Problem p[kMaxProblems];
@@ -538,16 +540,18 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
     bias0[e] = P.bias0 && n + e < P.N && !to_slab ? (float)((const T *)P.bias0)[n + e] : 0.f;
     bias1[e] = kParts == 2 && P.bias1 && n + e < P.N ? (float)((const T *)P.bias1)[n + e] : 0.f;
   }
-  // Whole rows of vectors (every column in one, rows at vector boundaries, no padding): buffer stores with 32-bit offsets;
-  // rows behind the last and columns behind N fall outside the descriptor's bound and are dropped.  Anything else goes
-  // element by element through put().
+  // Whole rows of vectors (every column in one, the rows' padding counted, and rows at vector boundaries): buffer stores with
+  // 32-bit offsets; rows behind the last and columns behind the padding fall outside the descriptor's bound and are dropped.
+  // Anything else goes element by element through put().  (1003 x 777 -> 2051, whose h, a, b, da and db are padded, fp16
+  // trained: element by element 143 us, like this 130.)
   using OutT = T;
-  const bool vectors = (P.N & 3) == 0 && P.pad <= P.N && (to_slab || whole);
-  const long ld_out = to_slab ? P.N : P.ldc;
+  const int cols = to_slab ? slab_ld(P.N) : max(P.N, P.pad);
+  const bool vectors = (cols & 3) == 0 && (to_slab || whole);
+  const long ld_out = to_slab ? slab_ld(P.N) : P.ldc;
   const int size_out = to_slab ? 4 : (int)sizeof(OutT);
   const int m_base = m0 + a_first;
   const auto bound = [&](long ld, int size) -> uint32_t {               // bytes from (m_base, 0) to the last column of the last row
-    const long bytes = ((long)(P.M - m_base - 1) * ld + P.N) * size;
+    const long bytes = ((long)(P.M - m_base - 1) * ld + cols) * size;
     return P.M <= m_base ? 0u : bytes > 0x7fffffffL ? 0x7fffffffu : (uint32_t)bytes;
   };
   const auto resource = [&](const void *base, long ld, int size) {
@@ -563,7 +567,7 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
     rx0 = resource(P.out0, P.ldaux, 4);
     rx1 = resource(P.out1, P.ldaux, 4);
   }
-  const bool exists = n < P.N;
+  const bool exists = n < cols;
   const uint32_t step_out = row_step * (uint32_t)(ld_out * size_out), step_aux = row_step * (uint32_t)(P.ldaux * 4);
   const uint32_t off_out = exists ? (uint32_t)(r_lane * ld_out + n) * size_out : 0x80000000u;
   const uint32_t off_aux = exists ? (uint32_t)(r_lane * P.ldaux + n) * 4 : 0x80000000u;
@@ -622,8 +626,9 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
           if constexpr (C::kind == kGateUp) {
             o0[u][e] = value[u * 4 + e] * v[u][kParts - 1][e];
           } else {
-            o0[u][e] = v[u][0][e] * x.b[u][e] * slope[u * 4 + e];
-            o1[u][e] = v[u][0][e] * value[u * 4 + e];
+            // (W_down's rows follow each other: behind the last column there is the next row's first)
+            o0[u][e] = n + e < P.N ? v[u][0][e] * x.b[u][e] * slope[u * 4 + e] : 0.f;
+            o1[u][e] = n + e < P.N ? v[u][0][e] * value[u * 4 + e] : 0.f;
           }
         }
     }
@@ -689,8 +694,7 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
           const int m = m_base + done * kRows + r_lane;
           if (m >= P.M) continue;
           T *row = (T *)P.c + (long)m * P.ldc;
-          if (to_slab) put<float>(P.slab + (long)slice * P.slab_stride + (long)m * P.N, n, P.N, 0, false, o0[u]);
-          else put<T>(row, n, P.N, P.pad, whole, o0[u]);
+          put<T>(row, n, P.N, P.pad, whole, o0[u]);
           if constexpr (C::kind == kGrad) put<T>((T *)P.c2 + (long)m * P.ldc, n, P.N, P.pad, whole, o1[u]);
           if constexpr (C::kind == kGateUp) {
             if (P.out0) {

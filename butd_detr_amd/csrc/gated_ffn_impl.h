@@ -152,14 +152,15 @@ template <typename T> __global__ __launch_bounds__(256) void copy_rows_kernel(co
 // ---- slabs of a split contraction -----------------------------------------------------------------------------------------
 struct Fold {
   const float *slab;
-  long stride;
+  long stride;                 // elements between slices
+  int ld;                      // ... and rows of a slice
   int split, M, N;
   void *c;
   long ldc;
   const void *bias;
   long first;
 };
-constexpr int kMaxFolds = 2 * kMaxProblems;
+constexpr int kMaxFolds = 2 * kMaxProblems + 1;
 struct Folds {
   Fold f[kMaxFolds];
   int count;
@@ -175,9 +176,9 @@ template <typename T> __global__ __launch_bounds__(256) void fold_kernel(const F
   const long m = q / quads;
   if (m >= F.M) return;
   const int n = (int)(q - m * quads) * 4;
-  const float *src = F.slab + m * F.N + n;
+  const float *src = F.slab + m * F.ld + n;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
-  if ((F.N & 3) == 0) {
+  if (((F.ld | F.stride) & 3) == 0) {                    // (rows padded to vectors: a column behind the last is read, not stored)
     f32x4 s = *(const f32x4 *)src;
 #pragma unroll 8
     for (int i = 1; i < F.split; ++i) s += *(const f32x4 *)(src + i * F.stride);      // in slice order: reproducible
@@ -415,14 +416,14 @@ template <typename T> struct Block {
     p.segments = 1;
     p.split = 1;
   }
-  static void add_fold(Folds &F, const float *slab, long stride, int split, int M, int N, void *c, long ldc, const void *bias) {
-    F.f[F.count++] = Fold{slab, stride, split, M, N, c, ldc, bias, F.blocks};
+  static void add_fold(Folds &F, const float *slab, long stride, int ld, int split, int M, int N, void *c, long ldc, const void *bias) {
+    F.f[F.count++] = Fold{slab, stride, ld, split, M, N, c, ldc, bias, F.blocks};
     F.blocks += ((long)M * ((N + 3) / 4) + 255) / 256;
   }
   static void add_folds(Folds &F, const Launch &L) {
     for (int i = 0; i < L.count; ++i) {
       const Problem &p = L.p[i];
-      if (p.split > 1) add_fold(F, p.slab, p.slab_stride, p.split, p.M, p.N, p.c, p.ldc, p.bias0);
+      if (p.split > 1) add_fold(F, p.slab, p.slab_stride, slab_ld(p.N), p.split, p.M, p.N, p.c, p.ldc, p.bias0);
     }
   }
   static hipError_t run_folds(const Folds &F, hipStream_t stream) {
@@ -443,7 +444,7 @@ template <typename T> struct Block {
       const int per = (steps + split - 1) / split;
       p.split = (steps + per - 1) / per;                 // every slice owns at least one step
       if (p.split > 1) {
-        p.slab_stride = ((long)p.M * p.N + 3) / 4 * 4;
+        p.slab_stride = (long)p.M * slab_ld(p.N);
         p.slab = (float *)ws.take(p.slab_stride * p.split * 4);
       }
     }
@@ -610,15 +611,13 @@ template <typename T> struct Block {
       hipLaunchKernelGGL((column_sum_kernel<T>), dim3((unsigned)blocks, (unsigned)S.chunks), dim3(256), 0, stream, S);
       if ((err = hipGetLastError()) != hipSuccess) return err;
     }
-    if (A.dx) {
-      if ((err = run_tiles<T, kPlain, kNN>(X, xc.size, stream)) != hipSuccess) return err;
-      if ((err = fold(X, stream)) != hipSuccess) return err;
-    }
+    if (A.dx && (err = run_tiles<T, kPlain, kNN>(X, xc.size, stream)) != hipSuccess) return err;
     if (W.count && (err = run_tiles<T, kPlain, kTN>(W, wc.size, stream)) != hipSuccess) return err;
-    // the weight gradients' slabs and the bias gradients' row chunks in one launch
+    // the slabs of dx and of the weight gradients and the bias gradients' row chunks in one launch
     Folds last{};
+    add_folds(last, X);
     add_folds(last, W);
-    for (int i = 0; i < S.count; ++i) add_fold(last, S.c[i].part, S.c[i].cols, S.chunks, 1, S.c[i].cols, S.c[i].out, S.c[i].cols, nullptr);
+    for (int i = 0; i < S.count; ++i) add_fold(last, S.c[i].part, S.c[i].cols, S.c[i].cols, S.chunks, 1, S.c[i].cols, S.c[i].out, S.c[i].cols, nullptr);
     return run_folds(last, stream);
   }
 };

@@ -4,7 +4,7 @@
 
 -- the gated variant of the FFN of the encoder / decoder layers (models/encoder_decoder_layers.py:110-122,315-323 build
 Linear-ReLU-Linear), for fp32, bf16 and fp16 tensors.  Forward is two launches (both projections, the activation and the
-product are one kernel), backward three to six.  Up to 16 rows -- a token each of a few sequences; up to 64 where the
+product are one kernel), backward three to seven.  Up to 16 rows -- a token each of a few sequences; up to 64 where the
 weights are small -- take kernels that do nothing but stream the weights.  The precision is the tensors' own (``fused_attention.set_compute_dtype`` does not apply):
 16-bit operands, everything between two products in 32 bits.  Checks, allocation and the autograd node are C++
 (binding/blocks_aten.cpp): a small layer is bound by the host.
