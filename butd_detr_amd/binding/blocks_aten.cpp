@@ -3,6 +3,7 @@
 // is bound by the host: as Python autograd functions over ctypes a forward + backward took about 145 us of it, the kernels
 // of 2048 rows x 288 take 25.
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -46,11 +47,27 @@ void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor value(const Maybe &t) { return t.has_value() ? *t : Tensor(); }
 Tensor contiguous(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
 
-bool wants_grad(std::initializer_list<Tensor> ts) {
-  if (!at::GradMode::is_enabled()) return false;
+bool wants_grad(std::initializer_list<Tensor> ts, const char *what) {
   for (const Tensor &t : ts)
-    if (t.defined() && t.requires_grad()) return true;
-  return false;
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), what, ": forward-mode derivatives are not implemented");
+  if (!at::GradMode::is_enabled()) return false;
+  bool wanted = false;
+  for (const Tensor &t : ts) wanted |= t.defined() && t.requires_grad();
+  if (!wanted) return false;
+  // A leaf whose gradient accumulator an eager graph keeps alive belongs to that graph's stream.  A backward pass captured
+  // elsewhere makes that stream wait for the capture; the default stream cannot, which ends the process: refused here.
+  const hipStream_t stream = (hipStream_t)stream_of(*ts.begin());
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (!stream || hipStreamIsCapturing(stream, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return true;
+  for (const Tensor &t : ts) {
+    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto owner = accumulator ? accumulator->stream() : std::nullopt;
+    TORCH_CHECK(!owner || c10::hip::HIPStreamMasqueradingAsCUDA(*owner).stream() != nullptr, what,
+                ": captured into a graph while an eager graph of the same leaves is alive on the default stream; release its "
+                "outputs first");
+  }
+  return true;
 }
 
 // What a backward pass hands back is not differentiable: under create_graph a second derivative raises instead of being zero.
@@ -191,9 +208,9 @@ Tensor gated_ffn(const Tensor &x, const Tensor &w_gate, const Tensor &w_up, cons
   if (b_up.has_value()) need("b_up", *b_up, {hidden});
   if (b_down.has_value()) need("b_down", *b_down, {width});
   TORCH_CHECK(x.is_cuda(), "CPU not supported");
-  TORCH_CHECK(x.numel() / width <= INT_MAX, "gated_ffn: at most 2^31 - 1 rows");
+  TORCH_CHECK(x.numel() / width <= 1L << 27, "gated_ffn: at most 2^27 rows");
   const Tensor bg = value(b_gate), bu = value(b_up), bd = value(b_down);
-  if (wants_grad({x, w_gate, w_up, w_down, bg, bu, bd}))
+  if (wants_grad({x, w_gate, w_up, w_down, bg, bu, bd}, "gated_ffn"))
     return GatedFfnNode::apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation);
   return ffn_forward(rows_of(x), rows_of(w_gate), rows_of(w_up), rows_of(w_down), contiguous(bg), contiguous(bu), contiguous(bd),
                      activation, false)
@@ -365,7 +382,7 @@ std::tuple<Maybe, Maybe> residual_norm(const Tensor &x, const Maybe &residual, c
   const Tensor r = value(residual), g = value(gate), p1 = value(w1), q1 = value(b1), p2 = value(w2), q2 = value(b2);
   const bool has_stream = r.defined() || g.defined() || post_kind;
   if (!has_stream && !pre_kind) return {Maybe(), Maybe()};
-  if (wants_grad({x, r, g, p1, q1, p2, q2})) {
+  if (wants_grad({x, r, g, p1, q1, p2, q2}, "residual_norm")) {
     variable_list out = ResidualNormNode::apply(x, residual, gate, w1, b1, w2, b2, post_kind, pre_kind, gate_kind, per_sample,
                                                 post_eps, pre_eps, scale);
     return {has_stream ? Maybe(out[0]) : Maybe(), pre_kind ? Maybe(out.back()) : Maybe()};

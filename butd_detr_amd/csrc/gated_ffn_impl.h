@@ -235,6 +235,7 @@ template <typename T> __global__ __launch_bounds__(256) void column_sum_kernel(c
 }
 // ---- plan -----------------------------------------------------------------------------------------------------------------
 constexpr int kCUs = 256;
+constexpr long kMaxBlocks = 0xffffffffL / 256;       // a launch has to stay below 2^32 threads
 constexpr long kMaxLd = 1L << 22;      // bytes between rows: 256 rows of a tile stay within a buffer descriptor's 2 GB
 
 struct Arena {                         // carves the workspace; with a null base it only counts
@@ -326,7 +327,7 @@ template <class C> inline hipError_t launch_tiles(Launch &L, hipStream_t stream)
   for (int i = 0; i < L.count; ++i) {
     Problem &p = L.p[i];
     const long tm = ((long)p.M + C::TM - 1) / C::TM, tn = ((long)p.N + nw - 1) / nw;
-    if (tm * tn > 0x7fffffffL - total) return hipErrorInvalidValue;
+    if (tm * tn > 0xffffffffL / C::kThreads - total) return hipErrorInvalidValue;
     p.tiles_m = (int)tm;
     p.tiles_n = (int)tn;
     p.first = (int)total;
@@ -389,7 +390,7 @@ template <typename T> struct Block {
     }
     hipError_t run(hipStream_t stream) {
       if (!L.count) return hipSuccess;
-      if (blocks > 0x7fffffffL) return hipErrorInvalidValue;
+      if (blocks > kMaxBlocks) return hipErrorInvalidValue;
       hipLaunchKernelGGL((copy_rows_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, L);
       return hipGetLastError();
     }
@@ -428,7 +429,7 @@ template <typename T> struct Block {
   }
   static hipError_t run_folds(const Folds &F, hipStream_t stream) {
     if (!F.count) return hipSuccess;
-    if (F.blocks > 0x7fffffffL) return hipErrorInvalidValue;
+    if (F.blocks > kMaxBlocks) return hipErrorInvalidValue;
     hipLaunchKernelGGL((fold_kernel<T>), dim3((unsigned)F.blocks), dim3(256), 0, stream, F);
     return hipGetLastError();
   }

@@ -14,10 +14,12 @@ int forced_tile = 0, forced_split = 0;
 
 namespace {
 
+constexpr long kMostRows = 1L << 27;     // (a launch of the smallest tiles stays below 2^32 threads)
+
 bool valid(const butd_gated_ffn_args *a, bool backward) {
   if (!a || a->dtype < BUTD_FFN_F32 || a->dtype > BUTD_FFN_F16) return false;
   if (a->activation < BUTD_FFN_SILU || a->activation > BUTD_FFN_SIGMOID) return false;
-  if (a->rows < 0 || a->rows > 0x7fffffffL || a->width < 1 || a->hidden < 1) return false;
+  if (a->rows < 0 || a->rows > kMostRows || a->width < 1 || a->hidden < 1) return false;
   // (offsets inside a tile's 256 rows have to fit 31 bits)
   constexpr long kMost = 1L << 20;
   if (a->width > kMost || a->hidden > kMost) return false;

@@ -139,14 +139,14 @@ template <int TPR> struct Group {
 };
 
 template <typename T, typename R, int TPR, Mode MODE>
-__global__ __launch_bounds__(Group<TPR>::kThreads, TPR == 1024 ? 8 : 1) void forward_kernel(const Args A) {
+__global__ __launch_bounds__(Group<TPR>::kThreads, TPR == 1024 ? 8 : 1) void forward_kernel(const Args A, const long row0) {
   __shared__ float sums[2][TPR / 64][1];
   __builtin_amdgcn_s_setprio(BUTD_MAIN_PRIO);
   RowSum<TPR, 1> row_sum{sums};
   const int sub = threadIdx.x / TPR, th = threadIdx.x % TPR, cols = A.cols;
   const int twice = MODE == kOverlap && th * N < cols ? max(th * N + N - cols, 0) : 0;
   const int c = th * N - twice, left = cols - c;
-  const long row = (long)blockIdx.x * Group<TPR>::kRows + sub, at = row * cols + c;
+  const long row = row0 + (long)blockIdx.x * Group<TPR>::kRows + sub, at = row * cols + c;
   if (row >= A.rows) return;                             // (whole waves, or the whole workgroup)
   // everything the row needs is on its way before the first sum
   float x[N], r[N], w1[N], b1[N], g[N];
@@ -426,28 +426,32 @@ struct Fold {
 struct Folds {
   Fold f[5];
   int n, cols, col_blocks;
+  long items;
 };
 template <typename T> __global__ __launch_bounds__(1024) void fold_kernel(const Folds L) {
-  int fi = 0;
-#pragma unroll
-  for (int i = 1; i < 5; ++i)
-    if (i < L.n && (long)blockIdx.x >= L.f[i].first) fi = i;
-  const Fold F = L.f[fi];
-  const long item = (long)blockIdx.x - F.first, o = item / L.col_blocks;
-  const int c = (int)(item - o * L.col_blocks) * 64 + (threadIdx.x & 63), sub = threadIdx.x >> 6;
-  float s = 0.f;
-  if (c < L.cols) {
-    const float *p = F.part + o * F.count * F.stride + c;
-#pragma unroll 4
-    for (long k = sub; k < F.count; k += 16) s += p[k * F.stride];
-  }
   __shared__ float sums[16][64];
-  sums[sub][threadIdx.x & 63] = s;
-  __syncthreads();
-  if (sub == 0 && c < L.cols) {
-    for (int k = 1; k < 16; ++k) s += sums[k][threadIdx.x];
-    if (F.f32) ((float *)F.out)[o * L.cols + c] = s;
-    else ((T *)F.out)[o * L.cols + c] = (T)s;
+  for (long at = blockIdx.x; at < L.items; at += gridDim.x) {
+    int fi = 0;
+#pragma unroll
+    for (int i = 1; i < 5; ++i)
+      if (i < L.n && at >= L.f[i].first) fi = i;
+    const Fold F = L.f[fi];
+    const long item = at - F.first, o = item / L.col_blocks;
+    const int c = (int)(item - o * L.col_blocks) * 64 + (threadIdx.x & 63), sub = threadIdx.x >> 6;
+    float s = 0.f;
+    if (c < L.cols) {
+      const float *p = F.part + o * F.count * F.stride + c;
+#pragma unroll 4
+      for (long k = sub; k < F.count; k += 16) s += p[k * F.stride];
+    }
+    __syncthreads();                                       // (the sums of the item before have been read)
+    sums[sub][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (sub == 0 && c < L.cols) {
+      for (int k = 1; k < 16; ++k) s += sums[k][threadIdx.x];
+      if (F.f32) ((float *)F.out)[o * L.cols + c] = s;
+      else ((T *)F.out)[o * L.cols + c] = (T)s;
+    }
   }
 }
 
@@ -478,6 +482,8 @@ bool valid(const Args *a, bool backward) {
   return true;
 }
 
+constexpr long kMaxBlocks = 1L << 21;
+
 // threads of a row: the smallest power of two of them that holds it, eight elements each
 template <typename F> hipError_t by_width(int cols, F &&f) {
   if (cols <= 64 * N) return f.template operator()<64>();
@@ -491,12 +497,18 @@ template <typename T, typename R> struct Forward {
   const Args &A;
   hipStream_t stream;
   template <int TPR> hipError_t operator()() {
-    const long blocks = (A.rows + Group<TPR>::kRows - 1) / Group<TPR>::kRows;
     auto *kernel = A.cols % N == 0 ? &forward_kernel<T, R, TPR, kWhole> : &forward_kernel<T, R, TPR, kOverlap>;
     if constexpr (TPR == 64)
       if (A.cols < N) kernel = &forward_kernel<T, R, TPR, kElements>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(Group<TPR>::kThreads), 0, stream, A);
-    return hipGetLastError();
+    // (a launch has to stay below 2^32 threads)
+    hipError_t err = hipSuccess;
+    for (long row0 = 0; row0 < A.rows && err == hipSuccess; row0 += kMaxBlocks * Group<TPR>::kRows) {
+      const long blocks = (A.rows - row0 + Group<TPR>::kRows - 1) / Group<TPR>::kRows;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks < kMaxBlocks ? blocks : kMaxBlocks)), dim3(Group<TPR>::kThreads), 0, stream, A,
+                         row0);
+      err = hipGetLastError();
+    }
+    return err;
   }
 };
 
@@ -572,8 +584,9 @@ template <typename T, typename R> struct Backward {
       add(P.gate_part, A.cols, P.slots / outputs, outputs, A.d_gate, A.gate_dtype);
     }
     if (!L.n) return hipSuccess;
-    if (first > 0x7fffffffL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((fold_kernel<T>), dim3((unsigned)first), dim3(1024), 0, stream, L);
+    L.items = first;
+    const long most = 1L << 16;
+    hipLaunchKernelGGL((fold_kernel<T>), dim3((unsigned)(first < most ? first : most)), dim3(1024), 0, stream, L);
     return hipGetLastError();
   }
 };

@@ -32,7 +32,7 @@ enum { BUTD_FFN_SILU = 0, BUTD_FFN_GELU = 1, BUTD_FFN_GELU_TANH = 2, BUTD_FFN_RE
 
 typedef struct {
   int dtype, activation;
-  long rows;                        /* tokens, 0 .. 2^31 - 1 */
+  long rows;                        /* tokens, 0 .. 2^27 */
   int width, hidden;                /* E, F: 1 .. 2^20 */
   const void *x;                    /* (rows, E) */
   const void *w_gate, *w_up;        /* (F, E) */

@@ -35,7 +35,7 @@ typedef struct {
   int stream_dtype;                 /* of residual, stream and their gradients: x_dtype or BUTD_NORM_F32 */
   int post_kind, pre_kind, gate_kind;
   int post_dtype, pre_dtype, gate_dtype;   /* of the norms' weight and bias, of gate: x_dtype or BUTD_NORM_F32 */
-  long rows, rows_per_sample;       /* rows = samples * rows_per_sample (read for BUTD_GATE_SAMPLE only) */
+  long rows, rows_per_sample;       /* 0 .. 2^31 - 1; rows = samples * rows_per_sample (read for BUTD_GATE_SAMPLE only) */
   int cols;
   float residual_scale, post_eps, pre_eps;
   const void *x, *residual;         /* residual may be NULL (taken as 0) */
@@ -50,6 +50,7 @@ typedef struct {
   void *d_x, *d_residual, *d_gate, *d_post_weight, *d_post_bias, *d_pre_weight, *d_pre_bias;
 } butd_residual_norm_args;
 
+/* Outputs share no memory with inputs or each other, here and in the backward call. */
 int butd_residual_norm_fwd(const butd_residual_norm_args *args, butd_stream_t stream);
 
 /* Bytes of device scratch (16-byte aligned) that the backward call with these arguments needs: a function of sizes, kinds

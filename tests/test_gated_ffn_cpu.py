@@ -111,3 +111,16 @@ def test_entry_points_check_their_arguments():
     for tile, split in [(32, 1), (64, 0), (64, 65), (0, 1), (-64, 1)]:
         assert lib.butd_gated_ffn_set_tile(tile, split) != 0
     assert lib.butd_gated_ffn_set_tile(0, 0) == 0
+
+
+def test_size_limits():
+    from butd_detr_amd import _hiplib
+    lib = _hiplib.load()
+    fwd = lambda a: lib.butd_gated_ffn_fwd_workspace(ctypes.byref(a))      # noqa: E731
+    assert fwd(_filled(lib, rows=1 << 27)) >= 0 and fwd(_filled(lib, rows=(1 << 27) + 1)) < 0
+    most = 1 << 20
+    assert fwd(_filled(lib, width=most)) >= 0 and fwd(_filled(lib, width=most + 1)) < 0
+    assert fwd(_filled(lib, hidden=most)) >= 0 and fwd(_filled(lib, hidden=most + 1)) < 0
+    a = _filled(lib)
+    a.ld_y = most + 1
+    assert fwd(a) < 0

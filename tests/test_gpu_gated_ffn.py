@@ -341,3 +341,90 @@ def test_second_derivatives_are_refused():
     (g,) = torch.autograd.grad(_apply(leaves, "silu"), [leaves["x"]], dy.requires_grad_(True), create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), [leaves["x"]])
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fw
+    t, dy = inputs(5, 8, 8, torch.float32)
+    with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        _apply({**t, "x": fw.make_dual(t["x"], torch.ones_like(t["x"]))}, "silu")
+
+
+def test_capture_beside_a_living_eager_graph_is_refused():
+    t, dy = inputs(70, 48, 40, torch.bfloat16)
+    leaves = {k: v.requires_grad_(True) for k, v in t.items()}
+    alive = _apply(leaves, "silu")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="eager graph"):
+            _apply(leaves, "silu")
+    (want,) = torch.autograd.grad(alive, [leaves["x"]], dy)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (got,) = torch.autograd.grad(_apply(leaves, "silu"), [leaves["x"]], dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows", [9, 200])
+def test_one_tensor_in_several_places_and_changed_in_place(rows):
+    """W_gate is W_up and x feeds its own layer's weights: gradients of the places add up; a weight that changed between the
+    passes is refused."""
+    from butd_detr_amd.gated_ffn import gated_ffn
+    t, dy = inputs(rows, 40, 40, torch.float32, bias=False)
+    want = reference({**t, "w_up": t["w_gate"]}, dy, "silu")
+    w = t["w_gate"].requires_grad_(True)
+    x, down = t["x"].requires_grad_(True), t["w_down"].requires_grad_(True)
+    y = gated_ffn(x, w, w, down)
+    g = torch.autograd.grad(y, [x, w, down], dy, retain_graph=True)
+    (vg, eg), (vu, eu) = want["d_w_gate"], want["d_w_up"]
+    both = (vg + vu, eg + eu + E32 * (vg + vu).abs())
+    check({"d_x": g[0], "d_w_gate": g[1], "d_w_down": g[2]}, {**want, "d_w_gate": both}, "shared")
+    again = torch.autograd.grad(y, [x, w, down], dy, retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(g, again))
+    with torch.no_grad():
+        down.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, [x], dy)
+
+
+def test_calls_from_several_threads():
+    import threading
+    jobs = [(inputs(rows, 96, 72, torch.bfloat16, seed=rows), kind) for rows, kind in ((3, "silu"), (130, "gelu"), (700, "relu"), (65, "sigmoid"))]
+    want = [run(t, dy, kind) for (t, dy), kind in jobs]
+    torch.cuda.synchronize()                                 # (their inputs come from this thread's stream)
+    got = [[] for _ in jobs]
+
+    def work(i):
+        (t, dy), kind = jobs[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i].append(run(t, dy, kind))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for w, runs in zip(want, got):
+        assert len(runs) == 5
+        for g in runs:
+            for k in w:
+                assert torch.equal(g[k], w[k]), k
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements between the first and the last row of h, a and b.  dy is zero but for the last 64 rows, so the
+    gradients are those of these rows alone."""
+    rows, width, hidden, last = 2_100_000, 16, 1040, 64
+    t, dy = inputs(rows, width, hidden, torch.bfloat16)
+    dy[:-last] = 0
+    tail = {k: (v[-last:] if k == "x" else v) for k, v in t.items()}
+    want = reference(tail, dy[-last:], "silu")
+    got = run(t, dy, "silu")
+    assert not got["d_x"][:-last].any()
+    check({k: (v[-last:] if k in ("y", "d_x") else v) for k, v in got.items()}, want, "last rows")

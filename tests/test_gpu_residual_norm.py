@@ -384,3 +384,69 @@ def test_a_stack_of_gated_blocks(rows, dtype):
     u = max(torch.finfo(dtype).eps / 2, 2.0 ** -20)          # (32 bits: the sums' own errors, 2^-20 of the norm)
     for got, want, count in list(zip(*outs, [7, 7])) + [(g, w, 14) for g, w in zip(*grads)]:
         assert float((got.double() - want).norm() / want.norm()) <= 4 * 3 * count ** 0.5 * u
+
+
+@pytest.mark.parametrize("batch, length", [(5, 1), (300, 2), (2, 700), (3, 1001)])
+@pytest.mark.parametrize("gate", ["channel", "sample", "element"])
+@pytest.mark.parametrize("cols", [9, 25, 601, 4097])
+def test_row_shares_of_odd_widths(cols, gate, batch, length):
+    """the last unit of a row overlaps its neighbour's"""
+    for dtype, stream in ((torch.float32, torch.float32), (torch.float16, torch.float16)):
+        t, norms, d = inputs(batch, length, cols, dtype, stream, "layer", "layer", gate)
+        check(run(t, norms, d, 1.25), reference(t, norms, d, 1.25), (cols, gate, batch, length, dtype))
+
+
+def _rows(t, d, a, b):
+    cut = lambda m: {k: (v[:, a:b].contiguous() if v.dim() == 3 else v) for k, v in m.items()}     # noqa: E731
+    return cut(t), cut(d)
+
+
+@pytest.mark.parametrize("rows, cols", [((1 << 23) + 5, 8), ((1 << 23) + 5, 7), (300_000, 8192)])
+def test_many_rows_and_offsets_beyond_32_bits(rows, cols):
+    """Rows do not depend on each other: the last and the first ones equal a call with these alone, bit for bit.  (The forward
+    pass launches 2^23 rows of up to 512 elements at a time.)"""
+    t, norms, d = inputs(1, rows, cols, torch.bfloat16, torch.bfloat16, "rms", "layer", "channel")
+    got = run(t, norms, d, 1.0)
+    for a, b in ((0, 70), (rows - 70, rows)):
+        alone = run(*(lambda p: (p[0], norms, p[1]))(_rows(t, d, a, b)), 1.0)
+        for k in ("stream", "normed", "d_x", "d_residual"):
+            assert torch.equal(got[k][:, a:b], alone[k]), (k, a)
+
+
+def test_many_samples():
+    """more sums of samples than workgroups of the kernel that rounds them"""
+    t, norms, d = inputs(70_000, 2, 24, torch.bfloat16, torch.float32, "layer", "rms", "sample")
+    check(run(t, norms, d, 1.0), reference(t, norms, d, 1.0), "samples")
+
+
+def test_one_tensor_in_two_places():
+    """x as its own residual: the gradients of both places add up"""
+    from butd_detr_amd.residual_norm import residual_norm
+    t, norms, d = inputs(2, 9, 100, torch.float32, torch.float32, "rms", "layer", None)
+    t["residual"] = t["x"]
+    want = reference(t, norms, d, 0.5)
+    x = t["x"].clone().requires_grad_(True)
+    out = residual_norm(x, x, post_norm=norms["post"], residual_scale=0.5, pre_norm=norms["pre"])
+    (g,) = torch.autograd.grad(out, [x], [d["stream"], d["normed"]])
+    (vx, ex), (vr, er) = want["d_x"], want["d_residual"]
+    check({"d_x": g}, {"d_x": (vx + vr, ex + er + 2.0 ** -24 * (vx.abs() + vr.abs()))}, "both")
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fw
+    t, norms, d = inputs(1, 3, 8, torch.float32, torch.float32, "rms", None, None)
+    with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        from butd_detr_amd.residual_norm import residual_norm
+        residual_norm(fw.make_dual(t["x"], t["x"].clone()), post_norm=norms["post"])
+
+
+def test_capture_beside_a_living_eager_graph_is_refused():
+    from butd_detr_amd.residual_norm import residual_norm
+    t, norms, d = inputs(2, 9, 100, torch.float32, torch.float32, "rms", "layer", None)
+    x = t["x"].requires_grad_(True)
+    alive = residual_norm(x, post_norm=norms["post"])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="eager graph"):
+            residual_norm(x, post_norm=norms["post"])
+    del alive
