@@ -3,7 +3,10 @@
 // Memory bound: forward reads x and residual and writes stream and normed, backward reads x, residual and the two arriving
 // gradients and writes two.  A row's values stay in registers from the load to the last use (both norms' statistics are
 // sums over registers, the deviations taken around the mean, not as a difference of squares), so each tensor is touched
-// once.  Rows of up to 512 elements belong to ONE wave and are reduced inside it; wider rows to a workgroup.  Rows of any
+// once.  Measured (16384 rows of 4096, bf16 on a 32-bit stream, RMSNorm on both sides, a gate per channel): forward 148 us,
+// backward 237 us, sums of the parameters' gradients 4.4 us -- 5.2, 5.1 TB/s, the rate of a large copy; 8192 rows of 8192 bf16
+// forward 98 us.  2048 rows of 288 fp32, the layers' own: 5.2, 9.3 and 3.4 us, launches more than bytes.
+// Rows of up to 512 elements belong to ONE wave and are reduced inside it; wider rows to a workgroup.  Rows of any
 // width and address, 16 bytes a lane.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -204,6 +207,8 @@ __global__ __launch_bounds__(Group<TPR>::kThreads, TPR == 1024 ? 8 : 1) void for
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------------
+// 180 to 220 registers a thread (four or five column sums of eight elements each, parameters, a row), so two waves a SIMD and
+// nobody to cover for a row's loads: the next row's are issued first (16384 rows of 4096: 307 -> 255 us).
 // A workgroup owns consecutive rows, [first, last) of one run of samples, and keeps its threads' column sums in registers:
 //   part[workgroup][4][cols]: d_post_weight, d_post_bias, d_pre_weight, d_pre_bias;   gate_part[slot][cols]
 // Gate per sample: the rows of a workgroup are either whole samples (slot = sample, written as each sample ends) or part of
@@ -414,7 +419,8 @@ __global__ __launch_bounds__(Group<TPR>::kThreads) void backward_kernel(const Ar
   }
 }
 
-// out[o][c] = sum over `count` partial rows, in order; 64 columns x 16 rows at a time
+// out[o][c] = sum over `count` partial rows, in a fixed order; 64 columns x 16 rows at a time (256 partial rows of 4 x 4096:
+// 4.4 us)
 struct Fold {
   const float *part;           // row k of output o at part + (o * count + k) * stride
   long stride;
