@@ -628,7 +628,8 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if constexpr (C::kind == kGateUp) {
-            o0[u][e] = value[u * 4 + e] * v[u][kParts - 1][e];
+            // (zeros behind the last column also where a row of x is infinite: the next product reads them)
+            o0[u][e] = n + e < P.N ? value[u * 4 + e] * v[u][kParts - 1][e] : 0.f;
           } else {
             // (W_down's rows follow each other: behind the last column there is the next row's first)
             o0[u][e] = n + e < P.N ? v[u][0][e] * x.b[u][e] * slope[u * 4 + e] : 0.f;

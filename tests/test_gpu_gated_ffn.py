@@ -428,3 +428,18 @@ def test_offsets_beyond_32_bits():
     got = run(t, dy, "silu")
     assert not got["d_x"][:-last].any()
     check({k: (v[-last:] if k in ("y", "d_x") else v) for k, v in got.items()}, want, "last rows")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, size", [(5, 64), (100, 64), (100, 128), (300, 256)])
+def test_an_infinite_row_stays_infinite(tile, rows, size, dtype):
+    """positive weights, one +inf in x, sigmoid: y of that row is +inf.  The hidden width fills no whole vector: what lies
+    behind its last column must not turn the sum into NaN."""
+    if rows > 16:
+        tile(size, 1)
+    t, _ = inputs(rows, 24, 37, dtype, bias=False)
+    t = {k: v.abs() + 0.125 for k, v in t.items()}
+    t["x"][1, 3] = float("inf")
+    for train in (False, True):
+        y = run(t, torch.zeros_like(t["x"]), "sigmoid", train=train)["y"]
+        assert torch.isposinf(y[1]).all() and torch.isfinite(y[0]).all() and torch.isfinite(y[2:]).all()
