@@ -197,9 +197,8 @@ struct Loader {
       kunit = ((lane & 7) ^ (PAIR ? key_pair(row) : key_natural(row))) * Num<T>::kVec;
     }
   }
-  // base: address of (first row, k0) resp. (k0, first row); bytes: what is readable from there; klimit = K - k0
-  __device__ inline void issue(char *lds, int wave, const char *base, long bytes, int klimit, int j0 = 0, int j1 = kChunks) const {
-    const uint32_t records = bytes > 0x7fffffffL ? 0x7fffffffu : (bytes < 0 ? 0u : (uint32_t)bytes);
+  // base: address of (first row, k0) resp. (k0, first row); records: bytes that are readable from there; klimit = K - k0
+  __device__ inline void issue(char *lds, int wave, const char *base, uint32_t records, int klimit, int j0 = 0, int j1 = kChunks) const {
     __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, records, 0x00020000);
     const bool live = !KC || kunit < klimit;             // a masked unit points past the bound and arrives as zeros
 #pragma unroll
@@ -408,15 +407,20 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
   if constexpr (C::kSegments) seek(it0 >= per_seg ? 1 : 0, (it0 >= per_seg ? it0 - per_seg : it0) * BK);
   else seek(0, it0 * BK);
   // (no branch around it: behind the last step nothing is readable, the stage arrives as zeros and costs no memory traffic)
+  uint32_t records_a, records_b;
+  auto prepare = [&]() {                                 // masks and selects: no branch
+    const uint32_t live = fetched < it1 ? 0xffffffffu : 0u;
+    records_a = (uint32_t)min(max(a_bytes, 0L), 0x7fffffffL) & live;
+    records_b = (uint32_t)min(max(b_bytes, 0L), 0x7fffffffL) & live;
+  };
   auto issue = [&](char *al, char *bl) {
-    const bool live = fetched < it1;
-    la.issue(al, wave, pa, live ? a_bytes : 0, left);
+    la.issue(al, wave, pa, records_a, left);
     if constexpr (kParts == 2) {
-      lb.issue(bl, wave, pb, live ? b_bytes : 0, left, 0, lb.kChunks / 2);
-      lb.issue(bl, wave, pb2, live ? b_bytes : 0, left, lb.kChunks / 2, lb.kChunks);
+      lb.issue(bl, wave, pb, records_b, left, 0, lb.kChunks / 2);
+      lb.issue(bl, wave, pb2, records_b, left, lb.kChunks / 2, lb.kChunks);
       pb2 += step_b;
     } else {
-      lb.issue(bl, wave, pb, live ? b_bytes : 0, left);
+      lb.issue(bl, wave, pb, records_b, left);
     }
     pa += step_a;
     pb += step_b;
@@ -492,13 +496,16 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
     read(al, bl, 1);
     multiply(0);
     interleave(0);
+    prepare();                                           // (not behind the barrier, where everything waits for it)
     fence();
     issue(al, bl);
     read(an, bn, 0);
     multiply(1);
     interleave(kLoads);
   };
+  prepare();
   issue(a_lds0, b_lds0);
+  prepare();
   fence();
   issue(a_lds1, b_lds1);
   read(a_lds0, b_lds0, 0);
