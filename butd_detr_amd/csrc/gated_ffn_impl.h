@@ -63,7 +63,8 @@ __global__ __launch_bounds__(NW * 64) void few_rows_kernel(const FewRows P) {
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[p][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   // kAhead pieces' loads are issued before the first of them is used (units past the contraction's end arrive as zeros)
-  constexpr int kAhead = MT == 4 ? 2 : 4;
+  // (more rows: fewer registers a piece and a second workgroup on the CU instead; 64 rows of 288 -> 256 fp32 15.4 -> 12.6 us)
+  constexpr int kAhead = MT == 1 ? 4 : MT == 2 ? 2 : 1;
   for (int k = wave * kStep; k < P.K; k += kAhead * NW * kStep) {
     u32x4 fw[kAhead][2][PARTS], fx[kAhead][2][MT];
 #pragma unroll
