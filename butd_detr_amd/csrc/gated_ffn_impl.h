@@ -5,6 +5,8 @@
 #include "ffn_tile.h"
 #include "zero_fill.h"
 
+#include <cmath>
+
 namespace ffn {
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------
@@ -271,7 +273,7 @@ extern int forced_tile, forced_split;
 // takes what one workgroup's step takes alone (latency) or what the multiplications of all workgroups of a CU take,
 // whichever is more; `fill` steps pass before the first and behind the last; the epilogue's bytes take the memory's time,
 // hidden in part where another workgroup of the CU computes meanwhile.  Slabs are written and read once, plus a launch.
-// No launch is faster than its operands' bytes at 4.5 TB/s.  Constants fitted to 120 measured launches of 16 shapes
+// The operands' bytes at 5.5 TB/s overlap with that in part (root of the squares' sum).  Constants fitted to 120 measured launches of 16 shapes
 // (1 .. 8192 rows x 200 .. 4096 x 256 .. 11264, both widths of types): the chosen tile was the fastest one in 3 of 4 and at
 // most 18 % slower in the rest.
 struct Shape {
@@ -295,6 +297,8 @@ template <typename T> inline TileChoice choose(const Shape *shapes, int count, l
   for (int i = 0; i < count; ++i) operands += (double)(shapes[i].M + shapes[i].N) * (double)k * segments * sizeof(T);
   for (int c = 0; c < (sizeof(T) == 2 ? 3 : 2); ++c) {
     const TileModel &m = models[c];
+    // (a tile with twice the rows that there are: 24 rows of 11264 -> 4096 bf16 24 us with the 128 tile, 18 with the 64)
+    if (count == 1 && shapes[0].M * 2 <= m.size && m.size > 64) break;
     const double area = (double)m.size * m.size, resident = kCUs * m.resident;
     double tiles = 0, elems = 0;
     for (int i = 0; i < count; ++i) {
@@ -312,9 +316,9 @@ template <typename T> inline TileChoice choose(const Shape *shapes, int count, l
         const double step = most * area * bk / m.rate * (sizeof(T) == 4 ? 1.0 : 0.6 + 0.4 * per_cu / most);
         return turn * (step > m.latency_us ? step : m.latency_us) + per_cu * area * bytes / 2e4 * (m.resident == 1 ? 1.2 : 0.6);
       };
-      double us = 3.0 + full * batch(resident);
+      double us = full * batch(resident);
       if (all > full * resident) us += batch(all - full * resident);
-      if (us < 3.0 + operands / 4.5e6) us = 3.0 + operands / 4.5e6;
+      us = 3.0 + sqrt(us * us + operands / 5.5e6 * (operands / 5.5e6));
       if (s > 1) us += 3.5 + elems * (4.0 * s + sizeof(T)) / 4.5e6;
       if (us < best.us) best = TileChoice{m.size, s, us};
     }
@@ -322,10 +326,13 @@ template <typename T> inline TileChoice choose(const Shape *shapes, int count, l
   return best;
 }
 
-// The streaming kernel's time: the weights once, and the rows again for every 16 columns (from L2; padded to 32 or 64).
+// The streaming kernel's time: the weights once and the rows again for every 16 columns (from L2; padded to 32 or 64), but
+// not less than one workgroup's way along the contraction, 128 bytes a wave at a time.
 template <typename T> inline double few_rows_us(long M, long N, long K, int parts) {
-  const double rows = M <= 32 ? 32 : 64;
-  return 3.0 + (double)N * K * sizeof(T) * parts / 5.6e6 + rows / 16 * (double)N * K * sizeof(T) / 6.5e6;
+  const double tiles = M <= 32 ? 2 : 4, weights = (double)N * K * sizeof(T);
+  const double all = weights * parts / 5.6e6 + tiles * weights / 6.5e6;
+  const double one = (double)((K * (long)sizeof(T) + 1023) / 1024) * (0.25 + 0.45 * tiles);
+  return 3.0 + (all > one ? all : one);
 }
 
 template <class C> inline hipError_t launch_tiles(Launch &L, hipStream_t stream) {
@@ -482,7 +489,8 @@ template <typename T> struct Block {
     hipError_t err;
     // Each product of up to 16 rows is streamed, and of 17 to 64 rows where tiles would be modelled slower or need copies
     // (bf16, 4096 -> 11264 -> 4096, streamed / tiles: 16 rows 64 / 73 us, 24 rows 81 / 73, 64 rows 132 / 79;
-    // 512 -> 2048 -> 512: 24 rows 10.9 / 14.2, 64 rows 16.8 / 14.4; 288 -> 256 -> 288: 64 rows 7.6 / 9.3)
+    // 512 -> 2048 -> 512: 24 rows 10.9 / 14.2, 64 rows 16.8 / 14.4; 288 -> 256 -> 288: 64 rows 7.6 / 9.3; fp32, 512 -> 2048
+    // -> 512, 64 rows 32.5 / 24.4, the first product streamed and the second on tiles 21.6)
     const Shape gs{M, 2L * F}, ds{M, E};
     const TileChoice gc = choose<T>(&gs, 1, E, 1, false, (A.a ? 8 + sizeof(T) : sizeof(T)) / 2.0),
                      dc = choose<T>(&ds, 1, F, 1, true, sizeof(T));
