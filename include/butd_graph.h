@@ -38,7 +38,7 @@ int butd_runtime_versions(int *runtime, int *driver);
  * the pool RCCL's own stream (ProcessGroupNCCL) and torch's default graph-capture stream come from too: the 33rd
  * "new" stream of a process IS one of the first 32 again.  A forked branch of a captured step that lands on RCCL's stream
  * puts that stream into capture mode while the process group's watchdog thread polls events recorded on it -> the
- * process aborts with hipErrorCapturedEvent (round 4, DESIGN.md 7.4 #6b; reproducer: scratch/stream_alias_probe.py).
+ * process aborts with hipErrorCapturedEvent.
  * The step's streams therefore never come from the pool (butd_detr_amd/graph_audit.py: own_stream). */
 int butd_stream_create(int priority, void **stream);
 int butd_stream_destroy(void *stream);
