@@ -450,3 +450,32 @@ def test_capture_beside_a_living_eager_graph_is_refused():
         with pytest.raises(RuntimeError, match="eager graph"):
             residual_norm(x, post_norm=norms["post"])
     del alive
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("deviation", [1.0, 0.03, 2.0 ** -11])
+def test_default_epsilon_against_the_module(dtype, deviation):
+    """nn.RMSNorm(eps=None): the module itself on the same tensor, before and after the block.  Both are off by their own
+    rounding and 32-bit statistics; a row of zeros is zero."""
+    from butd_detr_amd.residual_norm import residual_norm
+    g = torch.Generator(device="cuda").manual_seed(11)
+    m = nn.RMSNorm(288, device="cuda", dtype=dtype)
+    with torch.no_grad():
+        m.weight.copy_(1 + 0.2 * torch.randn(288, device="cuda", generator=g))
+    x = (deviation * torch.randn(9, 288, device="cuda", generator=g)).to(dtype)
+    x[4] = 0
+    u = torch.finfo(dtype).eps / 2 + E
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    with torch.no_grad():
+        want = m(x).double()
+        # the module may round twice: the normalised value, then its product with the weight
+        bound = want.abs() * (3 * u + u * u) + 3 * tiny
+        for got in (residual_norm(x, pre_norm=m)[1], residual_norm(x, post_norm=m)[0]):
+            assert float(((got.double() - want).abs() - bound).max()) <= 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_layer_norm_of_a_constant_row_is_zero(dtype):
+    from butd_detr_amd.residual_norm import residual_norm
+    x = torch.full((2, 40), 3.0, device="cuda", dtype=dtype)
+    assert float(residual_norm(x, pre_norm=nn.LayerNorm(40, device="cuda", dtype=dtype))[1].abs().max()) == 0.0

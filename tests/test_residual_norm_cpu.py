@@ -99,3 +99,18 @@ def test_entry_points_check_their_arguments():
     a = _filled()
     a.stats = 0
     assert need(a) < 0                                                          # the post norm's statistics are missing
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("params", [None, torch.float32])
+def test_default_epsilon_is_the_module_s_own(dtype, params):
+    """What nn.RMSNorm(eps=None) adds to the mean square of its input, solved from its own output: rows of 2^-12, where an
+    epsilon of the 16-bit types' would be thousands of mean squares."""
+    from butd_detr_amd.residual_norm import _norm
+    m = nn.RMSNorm(64, dtype=params or dtype)
+    x = torch.full((1, 64), 2.0 ** -12, dtype=dtype)
+    y = float(m(x)[0, 0])                                    # x / sqrt(x^2 + eps), rounded to at most 2^-9 of itself
+    eps = _norm("pre_norm", m, 64)[3]
+    want = 2.0 ** -12 / (2.0 ** -24 + eps) ** 0.5
+    assert abs(y - want) <= want * (torch.finfo(dtype).eps / 2 + 2.0 ** -20), (y, want, eps)
+    assert _norm("pre_norm", nn.RMSNorm(64, eps=0.5), 64)[3] == 0.5
