@@ -120,7 +120,8 @@ struct Problem {
   int M, N, K;                 // K: of one segment
   int segments;
   // kGateUp: b[0] / b[1] are W_gate / W_up of the ONE segment; c = h, aux0 / aux1 = a, b (32-bit) or null
-  // kGrad:   c = da, c2 = db, aux0 / aux1 = a, b
+  // kGrad:   c = da, c2 = db, aux0 / aux1 = a, b; out0 / out1 = column sums of da and db over each wave's rows,
+  //          (tiles_m * kWavesM, N), or null
   // kPlain:  c, or the 32-bit slab of slice s at slab + s * slab_stride (elements) when split > 1
   void *c, *c2;
   long ldc;                    // elements
@@ -139,6 +140,7 @@ struct Problem {
 };
 // rows of a slab are whole vectors
 __host__ __device__ inline int slab_ld(int n) { return (n + 3) & ~3; }
+constexpr int kWavesM = 2;                               // waves along m of every kGrad and kPlain tile
 constexpr int kMaxProblems = 3;
 struct Launch {
   Problem p[kMaxProblems];
@@ -353,7 +355,7 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
     const int rest = in - tn * gsz;
     tn += rest < 0 ? -1 : rest >= gsz ? 1 : 0;
   }
-  const int m0 = (first_m + in - tn * gsz) * C::TM, n0 = tn * (C::TN / kParts);
+  const int tm = first_m + in - tn * gsz, m0 = tm * C::TM, n0 = tn * (C::TN / kParts);
 
   const int per_seg = (P.K + BK - 1) / BK;
   const int it0 = slice * P.per_slice, it1 = min(P.steps, it0 + P.per_slice);
@@ -608,6 +610,8 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
       }
     }
   };
+  // kGrad: the lane's column sums of da and db, taken before their rounding (they are no operand of a product)
+  float sum0[4] = {0.f, 0.f, 0.f, 0.f}, sum1[4] = {0.f, 0.f, 0.f, 0.f};
   // element-wise part of a batch: v (kParts x 4 of each step) -> o0, o1
   auto combine = [&](float (&v)[U][kParts][4], const Aux &x, float (&o0)[U][4], float (&o1)[U][4]) {
     if constexpr (C::kind == kPlain) {
@@ -688,6 +692,15 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int done = chunk * kSteps + step + u;
+        if constexpr (C::kind == kGrad) {
+          if (m_base + done * kRows + r_lane < P.M) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              sum0[e] += o0[u][e];
+              sum1[e] += o1[u][e];
+            }
+          }
+        }
         if (vectors) {
           const uint32_t off = off_out + done * step_out;
           if (to_slab) store_buffer<float>(rc, off, o0[u]);
@@ -718,6 +731,26 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
       }
     }
     asm volatile("" ::: "memory");
+  }
+  if constexpr (C::kind == kGrad) {
+    static_assert(C::WM == kWavesM, "");
+    if (P.out0 || P.out1) {
+      // over the lanes that hold the same columns, in a fixed order
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int apart = kLanes; apart < 64; apart *= 2) {
+          sum0[e] += __shfl_xor(sum0[e], apart);
+          sum1[e] += __shfl_xor(sum1[e], apart);
+        }
+      const long at = ((long)tm * kWavesM + wm) * P.N + n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (r_lane == 0 && n + e < P.N) {
+          if (P.out0) P.out0[at + e] = sum0[e];
+          if (P.out1) P.out1[at + e] = sum1[e];
+        }
+    }
   }
 }
 

@@ -9,7 +9,9 @@
  *     dW_gate = da^T x   dW_up = db^T x            dW_down = dy^T h     bias gradients = column sums of da, db, dy
  * Both projections, the activation and the product are ONE kernel; so are dh with the activation's derivative, the two
  * products of dx, and the three weight gradients.  16-bit tensors: operands as they are, accumulation, biases, activation and
- * its derivative in 32 bits, h / da / db rounded once to the tensors' type (they are operands of the next product).
+ * its derivative in 32 bits, h / da / db rounded once to the tensors' type where they are operands of the next product (fp16:
+ * an h beyond 65504 is infinite, of da and db nothing below 2^-25 is left, as between the linear layers of an fp16 model);
+ * the bias gradients are sums of the unrounded da and db.
  * No atomics: results are bit-reproducible.
  *
  * Row-major, last dimension contiguous, leading strides (ld_*) in ELEMENTS; device pointers; asynchronous launches on

@@ -443,3 +443,53 @@ def test_an_infinite_row_stays_infinite(tile, rows, size, dtype):
     for train in (False, True):
         y = run(t, torch.zeros_like(t["x"]), "sigmoid", train=train)["y"]
         assert torch.isposinf(y[1]).all() and torch.isfinite(y[0]).all() and torch.isfinite(y[2:]).all()
+
+
+class _Rounded(torch.autograd.Function):
+    """rounds to ``dtype`` what goes forward and / or what comes back, values held in 64 bits"""
+
+    @staticmethod
+    def forward(ctx, v, dtype, forth, back):
+        ctx.dtype, ctx.back = dtype, back
+        return v.to(dtype).double() if forth else v.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        return (g.to(ctx.dtype).double() if ctx.back else g), None, None, None
+
+
+def emulated(t, dy, kind):
+    """The block in 64 bits with the roundings of include/butd_gated_ffn.h and no others: h forward, da and db backward --
+    operands of the next product -- and every output.  The bias gradients are sums of the unrounded da and db."""
+    dtype = t["x"].dtype
+    p = {k: v.detach().double().requires_grad_(True) for k, v in t.items()}
+    a, b = (_Rounded.apply(p["x"] @ p[w].t(), dtype, False, True) + p[v] for w, v in (("w_gate", "b_gate"), ("w_up", "b_up")))
+    if kind == "sigmoid":
+        v = torch.sigmoid(a)
+    elif kind == "gelu":
+        v = 0.5 * a * torch.erfc(-a * 0.5 ** 0.5)
+    else:
+        v = a * torch.sigmoid(a)
+    h = _Rounded.apply(v * b, dtype, True, False)
+    y = h @ p["w_down"].t() + p["b_down"]
+    grads = torch.autograd.grad(y, list(p.values()), dy.double())
+    return {k: v.detach().to(dtype) for k, v in {"y": y, **{"d_" + n: g for n, g in zip(p, grads)}}.items()}
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [(5, 256, 512), (40, 136, 264), (700, 288, 256), (1100, 200, 300), (2048, 77, 130)])
+def test_the_documented_roundings_and_no_others(size, dtype):
+    """Against ``emulated``, relative to an output's norm.  What is left are the 32-bit errors in front of each rounding, 2^-20
+    of the value: a value rounds the other way where it lies that close to a border between two of its neighbours 2 u apart,
+    a share of 2^-20 / u of all values, and is then off by 2 u.  The root mean square of one such stage is 2 u sqrt(2^-20 / u),
+    of the at most three stages on an output's way sqrt(3) times that: u / 18 for bf16, u / 6.5 for fp16 (u = 2^-8, 2^-11).
+    One rounding too many or one too few is at least u / sqrt(6) (a mantissa anywhere in [1, 2), an error anywhere in
+    [-u, u])."""
+    for kind in ("silu", "gelu", "sigmoid"):               # (the smooth ones: no slope jumps within an error of a)
+        t, dy = inputs(*size, dtype)
+        got, want = run(t, dy, kind), emulated(t, dy, kind)
+        u = torch.finfo(dtype).eps / 2
+        limit = 2 * u * (3 * 2.0 ** -20 / u) ** 0.5
+        for k in want:
+            far = float((got[k].double() - want[k].double()).norm() / want[k].double().norm())
+            assert far <= limit, (size, kind, k, far / u, limit / u)
