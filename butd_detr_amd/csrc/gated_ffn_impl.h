@@ -254,8 +254,14 @@ constexpr int kCUs = 256;
 constexpr long kMaxBlocks = 0xffffffffL / 256;       // a launch has to stay below 2^32 threads
 constexpr long kMaxLd = 1L << 22;      // bytes between rows: 256 rows of a tile stay within a buffer descriptor's 2 GB
 
+// what butd_gated_ffn_set_tile asks for, read once a call: a plan is counted and carried out with one setting.  0: the rule
+struct Forced {
+  int tile, split;
+};
+
 struct Arena {                         // carves the workspace; with a null base it only counts
   char *base;
+  Forced forced;
   long used = 0;
   void *take(long bytes) {
     char *p = base ? base + used : nullptr;
@@ -270,9 +276,6 @@ struct TileChoice {
   int size, split;                     // 256, 128 or 64
   double us;                           // modelled
 };
-
-// butd_gated_ffn_set_tile: (0, 0) = the rule below
-extern int forced_tile, forced_split;
 
 // Which tile, and into how many slices the contraction is cut (products whose slabs can be folded only): the smallest of the
 // modelled times.  The tiles go round the chip in batches of 256 CUs x as many workgroups as a CU holds.  A step of a batch
@@ -290,8 +293,8 @@ struct TileModel {
   double latency_us, rate, fill;       // rate: multiply-adds per CU and microsecond with all CUs at work
   int resident;                        // workgroups of a CU
 };
-template <typename T> inline TileChoice choose(const Shape *shapes, int count, long k, int segments, bool can_split, double epilogue_bytes) {
-  if (forced_tile) return TileChoice{sizeof(T) == 4 && forced_tile == 256 ? 128 : forced_tile, can_split ? forced_split : 1, 0.0};
+template <typename T> inline TileChoice choose(Forced forced, const Shape *shapes, int count, long k, int segments, bool can_split, double epilogue_bytes) {
+  if (forced.tile) return TileChoice{sizeof(T) == 4 && forced.tile == 256 ? 128 : forced.tile, can_split ? forced.split : 1, 0.0};
   static const TileModel models16[3] = {{64, 0.49, 1.15e6, 2.0, 4}, {128, 0.65, 1.75e6, 3.0, 2}, {256, 1.2, 2.4e6, 3.0, 1}};
   static const TileModel models32[2] = {{64, 0.60, 0.245e6, 1.5, 4}, {128, 2.0, 0.258e6, 1.5, 2}};
   static const int splits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
@@ -498,9 +501,9 @@ template <typename T> struct Block {
     // 512 -> 2048 -> 512: 24 rows 10.9 / 14.2, 64 rows 16.8 / 14.4; 288 -> 256 -> 288: 64 rows 7.6 / 9.3; fp32, 512 -> 2048
     // -> 512, 64 rows 32.5 / 24.4, the first product streamed and the second on tiles 21.6)
     const Shape gs{M, 2L * F}, ds{M, E};
-    const TileChoice gc = choose<T>(&gs, 1, E, 1, false, (A.a ? 8 + sizeof(T) : sizeof(T)) / 2.0),
-                     dc = choose<T>(&ds, 1, F, 1, true, sizeof(T));
-    const bool few = M <= kFewRows && !forced_tile;
+    const TileChoice gc = choose<T>(ws.forced, &gs, 1, E, 1, false, (A.a ? 8 + sizeof(T) : sizeof(T)) / 2.0),
+                     dc = choose<T>(ws.forced, &ds, 1, F, 1, true, sizeof(T));
+    const bool few = M <= kFewRows && !ws.forced.tile;
     const bool stream_in = few && (M <= 16 || !direct_in(A) || few_rows_us<T>(M, F, E, 2) <= gc.us);
     const bool stream_out = few && (M <= 16 || !Packer::direct(A.w_down, A.ld_down, F) || few_rows_us<T>(M, E, F, 1) <= dc.us);
     Packer pk(ws);
@@ -579,7 +582,7 @@ template <typename T> struct Block {
       g.c = (void *)da.p; g.c2 = (void *)db.p; g.ldc = A.ld_h; g.pad = (int)A.ld_h;
       g.aux0 = A.a; g.aux1 = A.b; g.ldaux = A.ld_h;
       const Shape s{M, F};
-      gc = choose<T>(&s, 1, E, 1, false, 8 + 2 * sizeof(T));
+      gc = choose<T>(ws.forced, &s, 1, E, 1, false, 8 + 2 * sizeof(T));
     }
     if (A.dx) {
       X.count = 1;
@@ -590,7 +593,7 @@ template <typename T> struct Block {
       p.M = M; p.N = E; p.K = F;
       p.c = A.dx; p.ldc = A.ld_dx;
       const Shape s{M, E};
-      xc = choose<T>(&s, 1, F, 2, true, sizeof(T));
+      xc = choose<T>(ws.forced, &s, 1, F, 2, true, sizeof(T));
       slabs(X, xc.split, ws);
     }
     Shape ws_shapes[3];
@@ -605,7 +608,7 @@ template <typename T> struct Block {
     if (A.dw_up) weight(db, x, F, E, A.dw_up);
     if (A.dw_down) weight(dy, Operand{A.h, A.ld_h}, E, F, A.dw_down);
     if (W.count) {
-      wc = choose<T>(ws_shapes, W.count, M, 1, true, sizeof(T));
+      wc = choose<T>(ws.forced, ws_shapes, W.count, M, 1, true, sizeof(T));
       slabs(W, wc.split, ws);
     }
     // bias gradients: column sums of da, db, dy in row chunks

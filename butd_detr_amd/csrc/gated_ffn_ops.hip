@@ -1,6 +1,8 @@
 // gated_ffn_ops.hip -- entry points of include/butd_gated_ffn.h: checks of the arguments, dispatch on the tensors' type.
 #include "gated_ffn_impl.h"
 
+#include <atomic>
+
 #define BUTD_FFN_DECLARE(T)                                                                            \
   hipError_t butd_ffn_forward_##T(const butd_gated_ffn_args &, ffn::Arena &, bool, hipStream_t);       \
   hipError_t butd_ffn_backward_##T(const butd_gated_ffn_args &, ffn::Arena &, bool, hipStream_t);
@@ -8,11 +10,13 @@ BUTD_FFN_DECLARE(f32)
 BUTD_FFN_DECLARE(bf16)
 BUTD_FFN_DECLARE(f16)
 
-namespace ffn {
-int forced_tile = 0, forced_split = 0;
-}
-
 namespace {
+
+std::atomic<int> tuned{0};               // butd_gated_ffn_set_tile: tile + 1024 split as one value
+ffn::Forced forced() {
+  const int v = tuned.load(std::memory_order_relaxed);
+  return ffn::Forced{v & 1023, v >> 10};
+}
 
 constexpr long kMostRows = 1L << 27;     // (a launch of the smallest tiles stays below 2^32 threads)
 
@@ -46,18 +50,19 @@ hipError_t dispatch(const butd_gated_ffn_args &a, ffn::Arena &ws, bool run, hipS
   }
 }
 
-long workspace(const butd_gated_ffn_args *a, bool backward) {
+long workspace(const butd_gated_ffn_args *a, bool backward, ffn::Forced setting) {
   if (!valid(a, backward)) return -(long)hipErrorInvalidValue;
-  ffn::Arena ws{nullptr};
+  ffn::Arena ws{nullptr, setting};
   const hipError_t err = dispatch(*a, ws, false, nullptr, backward);
   return err == hipSuccess ? ws.used : -(long)err;
 }
 
 int execute(const butd_gated_ffn_args *a, void *ws_ptr, long ws_bytes, butd_stream_t stream, bool backward) {
-  const long need = workspace(a, backward);
+  const ffn::Forced setting = forced();
+  const long need = workspace(a, backward, setting);
   if (need < 0) return (int)-need;
   if (need > 0 && (!ws_ptr || ws_bytes < need || ((uintptr_t)ws_ptr & 15))) return (int)hipErrorInvalidValue;
-  ffn::Arena ws{(char *)ws_ptr};
+  ffn::Arena ws{(char *)ws_ptr, setting};
   return (int)dispatch(*a, ws, true, (hipStream_t)stream, backward);
 }
 
@@ -71,16 +76,15 @@ long butd_gated_ffn_ld_hidden(int dtype, int hidden) {
 }
 int butd_gated_ffn_set_tile(int tile, int split) {
   if (tile == 0 && split == 0) {
-    ffn::forced_tile = ffn::forced_split = 0;
+    tuned.store(0, std::memory_order_relaxed);
     return 0;
   }
   if ((tile != 64 && tile != 128 && tile != 256) || split < 1 || split > 64) return (int)hipErrorInvalidValue;
-  ffn::forced_tile = tile;
-  ffn::forced_split = split;
+  tuned.store(tile + 1024 * split, std::memory_order_relaxed);
   return 0;
 }
-long butd_gated_ffn_fwd_workspace(const butd_gated_ffn_args *args) { return workspace(args, false); }
-long butd_gated_ffn_bwd_workspace(const butd_gated_ffn_args *args) { return workspace(args, true); }
+long butd_gated_ffn_fwd_workspace(const butd_gated_ffn_args *args) { return workspace(args, false, forced()); }
+long butd_gated_ffn_bwd_workspace(const butd_gated_ffn_args *args) { return workspace(args, true, forced()); }
 int butd_gated_ffn_fwd(const butd_gated_ffn_args *args, void *ws, long ws_bytes, butd_stream_t stream) {
   return execute(args, ws, ws_bytes, stream, false);
 }

@@ -63,8 +63,9 @@ typedef struct {
 long butd_gated_ffn_ld_hidden(int dtype, int hidden);
 
 /* Tuning hook: the tile (64, 128 or 256 rows and columns of a product; 256 is 128 for fp32) and the slices of the
- * contraction (1 .. 64, where a product can be split) of every following call; (0, 0) returns to the built-in rule.  The
- * workspace functions follow it.  Returns 0 or hipErrorInvalidValue.  Not thread-safe. */
+ * contraction (1 .. 64, where a product can be split) of every following call of the process; (0, 0) returns to the built-in
+ * rule.  A call reads it once.  The workspace functions follow it too: a call whose workspace was counted under another setting
+ * that needs less refuses it.  Returns 0 or hipErrorInvalidValue. */
 int butd_gated_ffn_set_tile(int tile, int split);
 
 /* Bytes of device scratch (16-byte aligned) that the call with these arguments needs: a function of dtype, sizes, strides,

@@ -124,3 +124,42 @@ def test_size_limits():
     a = _filled(lib)
     a.ld_y = most + 1
     assert fwd(a) < 0
+
+
+_HOOK_WHILE_PLANNING = """
+import ctypes, sys, threading
+sys.path.insert(0, {root!r})
+from butd_detr_amd import _hiplib
+from tests.test_gated_ffn_cpu import _filled
+lib = _hiplib.load()
+a = _filled(lib, rows=4096, width=512, hidden=2048)
+a.a, a.b, a.dy, a.dx, a.ld_dy, a.ld_dx, a.dw_gate, a.dw_up, a.dw_down = 4096, 8192, 12288, 16384, 512, 512, 4096, 4096, 4096
+need = lambda: lib.butd_gated_ffn_bwd_workspace(ctypes.byref(a))
+known = {{need()}}
+lib.butd_gated_ffn_set_tile(64, 48)
+known.add(need())
+assert len(known) == 2 and min(known) > 0
+done = threading.Event()
+def turn():
+    while not done.is_set():
+        lib.butd_gated_ffn_set_tile(0, 0)
+        lib.butd_gated_ffn_set_tile(64, 48)
+threads = [threading.Thread(target=turn) for _ in range(2)]
+for t in threads:
+    t.start()
+seen = {{need() for _ in range(200000)}}
+done.set()
+for t in threads:
+    t.join()
+assert seen <= known, (seen, known)
+"""
+
+
+def test_a_plan_is_made_of_one_setting_of_the_tuning_hook():
+    """The hook set by other threads while a plan is made: the plan is the one setting's or the other's, never a mixture."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", _HOOK_WHILE_PLANNING.format(root=root)], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0, (out.returncode, out.stderr[-1000:])
