@@ -219,6 +219,7 @@ class GatedFfnArgs(ctypes.Structure):
 
 
 GATED_FFN_SYMBOLS = {
+    "butd_gated_ffn_args_size": (_c_long, []),
     "butd_gated_ffn_ld_hidden": (_c_long, [_c_int, _c_int]),
     "butd_gated_ffn_set_tile": (_c_int, [_c_int, _c_int]),
     "butd_gated_ffn_fwd_workspace": (_c_long, [ctypes.POINTER(GatedFfnArgs)]),
@@ -243,6 +244,7 @@ class ResidualNormArgs(ctypes.Structure):
 
 
 RESIDUAL_NORM_SYMBOLS = {
+    "butd_residual_norm_args_size": (_c_long, []),
     "butd_residual_norm_fwd": (_c_int, [ctypes.POINTER(ResidualNormArgs), _P]),
     "butd_residual_norm_bwd_workspace": (_c_long, [ctypes.POINTER(ResidualNormArgs)]),
     "butd_residual_norm_bwd": (_c_int, [ctypes.POINTER(ResidualNormArgs), _P, _c_long, _P]),
@@ -285,6 +287,10 @@ def load():
             raise HipLibraryMissing(f"{LIB_PATH} does not export {name}") from e
         fn.restype = res
         fn.argtypes = args
+    for struct, size in ((GatedFfnArgs, lib.butd_gated_ffn_args_size()), (ResidualNormArgs, lib.butd_residual_norm_args_size())):
+        if ctypes.sizeof(struct) != size:
+            raise HipLibraryMissing(f"{LIB_PATH}: {struct.__name__} has {size} bytes there, {ctypes.sizeof(struct)} here: "
+                                    "build it again with `python -m butd_detr_amd.build`")
     _lib = lib
     return lib
 

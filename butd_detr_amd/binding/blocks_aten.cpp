@@ -395,6 +395,10 @@ std::tuple<Maybe, Maybe> residual_norm(const Tensor &x, const Maybe &residual, c
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  // (the argument structs go by pointer: their layout has to be the library's)
+  TORCH_CHECK(butd_gated_ffn_args_size() == (long)sizeof(butd_gated_ffn_args) &&
+                  butd_residual_norm_args_size() == (long)sizeof(butd_residual_norm_args),
+              "butd_blocks_aten and libbutd_detr_hip.so were built from different headers: python -m butd_detr_amd.binding.build");
   m.def("gated_ffn", &gated_ffn, py::call_guard<py::gil_scoped_release>());
   m.def("residual_norm", &residual_norm, py::call_guard<py::gil_scoped_release>());
 }

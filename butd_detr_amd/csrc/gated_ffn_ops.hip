@@ -70,6 +70,7 @@ int execute(const butd_gated_ffn_args *a, void *ws_ptr, long ws_bytes, butd_stre
 
 extern "C" {
 
+long butd_gated_ffn_args_size(void) { return (long)sizeof(butd_gated_ffn_args); }
 long butd_gated_ffn_ld_hidden(int dtype, int hidden) {
   const long vec = dtype == BUTD_FFN_F32 ? 4 : 8;
   return ((long)hidden + vec - 1) / vec * vec;

@@ -621,6 +621,8 @@ Args simplified(const Args &a) {
 
 extern "C" {
 
+long butd_residual_norm_args_size(void) { return (long)sizeof(butd_residual_norm_args); }
+
 int butd_residual_norm_fwd(const butd_residual_norm_args *args, butd_stream_t stream) {
   if (!valid(args, false)) return (int)hipErrorInvalidValue;
   if (args->rows == 0) return 0;

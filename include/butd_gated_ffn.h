@@ -59,6 +59,9 @@ typedef struct {
   void *db_gate, *db_up, *db_down;
 } butd_gated_ffn_args;
 
+/* sizeof(butd_gated_ffn_args) in the library: a caller that was compiled against another header finds out */
+long butd_gated_ffn_args_size(void);
+
 /* elements between the rows of h, a and b */
 long butd_gated_ffn_ld_hidden(int dtype, int hidden);
 

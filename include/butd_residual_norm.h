@@ -50,6 +50,9 @@ typedef struct {
   void *d_x, *d_residual, *d_gate, *d_post_weight, *d_post_bias, *d_pre_weight, *d_pre_bias;
 } butd_residual_norm_args;
 
+/* sizeof(butd_residual_norm_args) in the library: a caller that was compiled against another header finds out */
+long butd_residual_norm_args_size(void);
+
 /* Outputs share no memory with inputs or each other, here and in the backward call. */
 int butd_residual_norm_fwd(const butd_residual_norm_args *args, butd_stream_t stream);
 
