@@ -34,7 +34,6 @@
 namespace ffn {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -529,7 +528,7 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
   const int slot = wave * kChunkBytes / C::kA;
   char *mine = (slot == 0 ? a_lds0 : slot == 1 ? b_lds0 : slot == 2 ? a_lds1 : b_lds1) + wave * kChunkBytes % C::kA;
   const int i16 = lane & 15, g = lane >> 4;
-  const bool whole = (P.ldc % 4 == 0) && ((uintptr_t)P.c & 15) == 0 && ((uintptr_t)P.c2 & 15) == 0;
+  const bool whole = (P.ldc % 4 == 0) && ((uintptr_t)P.c & 15) == 0;
   const bool to_slab = C::kind == kPlain && P.split > 1;
   constexpr int kLanes = kQuads / kParts, kRows = 64 / kLanes;                    // lanes of a row, rows of a step
   constexpr int kSteps = CT * 16 / kRows, U = kSteps < 4 ? kSteps : 4;            // steps of a chunk, of a batch
@@ -555,11 +554,12 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
   }
   // Whole rows of vectors (every column in one, the rows' padding counted, and rows at vector boundaries): buffer stores with
   // 32-bit offsets; rows behind the last and columns behind the padding fall outside the descriptor's bound and are dropped.
-  // Anything else goes element by element through put().  (1003 x 777 -> 2051, whose h, a, b, da and db are padded, fp16
+  // Of h, a, b, da and db that is every case (the launch checks it); y, dx and weight gradients of other widths or addresses go
+  // element by element through put().  (1003 x 777 -> 2051, whose h, a, b, da and db are padded, fp16
   // trained: element by element 143 us, like this 130.)
   using OutT = T;
   const int cols = to_slab ? slab_ld(P.N) : max(P.N, P.pad);
-  const bool vectors = (cols & 3) == 0 && (to_slab || whole);
+  const bool vectors = C::kind != kPlain || ((cols & 3) == 0 && (to_slab || whole));
   const long ld_out = to_slab ? slab_ld(P.N) : P.ldc;
   const int size_out = to_slab ? 4 : (int)sizeof(OutT);
   const int m_base = m0 + a_first;
@@ -593,20 +593,9 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
     if constexpr (C::kind == kGrad) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (vectors) {
-          const uint32_t off = off_aux + (step + u) * step_aux;
-          x.a[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx0, off, 0, 0));
-          x.b[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx1, off, 0, 0));
-        } else {
-          const int m = m_base + (step + u) * kRows + r_lane;
-          x.a[u] = x.b[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (m < P.M && n + e < P.N) {
-              x.a[u][e] = P.aux0[(long)m * P.ldaux + n + e];
-              x.b[u][e] = P.aux1[(long)m * P.ldaux + n + e];
-            }
-        }
+        const uint32_t off = off_aux + (step + u) * step_aux;
+        x.a[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx0, off, 0, 0));
+        x.b[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx1, off, 0, 0));
       }
     }
   };
@@ -715,18 +704,9 @@ template <class C> __global__ __launch_bounds__(C::kThreads) void tile_kernel(co
               store_buffer<float>(rx1, aux, v[u][kParts - 1]);
             }
           }
-        } else {
+        } else if constexpr (C::kind == kPlain) {
           const int m = m_base + done * kRows + r_lane;
-          if (m >= P.M) continue;
-          T *row = (T *)P.c + (long)m * P.ldc;
-          put<T>(row, n, P.N, P.pad, whole, o0[u]);
-          if constexpr (C::kind == kGrad) put<T>((T *)P.c2 + (long)m * P.ldc, n, P.N, P.pad, whole, o1[u]);
-          if constexpr (C::kind == kGateUp) {
-            if (P.out0) {
-              put<float>(P.out0 + (long)m * P.ldaux, n, P.N, 0, true, v[u][0]);
-              put<float>(P.out1 + (long)m * P.ldaux, n, P.N, 0, true, v[u][kParts - 1]);
-            }
-          }
+          if (m < P.M) put<T>((T *)P.c + (long)m * P.ldc, n, P.N, 0, whole, o0[u]);
         }
       }
     }

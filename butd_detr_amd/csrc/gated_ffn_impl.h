@@ -46,9 +46,9 @@ struct FewRows {
   long ldaux;
 };
 
-template <typename T, int PARTS, int MT, bool AL, int NW>
-__global__ __launch_bounds__(NW * 64) void few_rows_kernel(const FewRows P) {
-  constexpr int kVec = Num<T>::kVec, kStep = 8 * kVec;   // 128 bytes of a row
+template <typename T, int PARTS, int MT, bool AL>
+__global__ __launch_bounds__(512) void few_rows_kernel(const FewRows P) {
+  constexpr int NW = 8, kVec = Num<T>::kVec, kStep = 8 * kVec;   // 128 bytes of a row
   __shared__ f32x4 part[NW][PARTS * MT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16;
@@ -350,6 +350,11 @@ template <class C> inline hipError_t launch_tiles(Launch &L, hipStream_t stream)
   int slices = 1;
   for (int i = 0; i < L.count; ++i) {
     Problem &p = L.p[i];
+    if constexpr (C::kind != kPlain) {                   // the epilogue of h, a, b, da and db knows whole vectors only
+      const uintptr_t at = (uintptr_t)p.c | (uintptr_t)p.c2 | (uintptr_t)p.aux0 | (uintptr_t)p.aux1 |
+                           (C::kind == kGateUp ? (uintptr_t)p.out0 | (uintptr_t)p.out1 : 0);
+      if (p.pad < p.N || (p.pad | p.ldc | p.ldaux) & 3 || at & 15) return hipErrorInvalidValue;
+    }
     const long tm = ((long)p.M + C::TM - 1) / C::TM, tn = ((long)p.N + nw - 1) / nw;
     if (tm * tn > 0xffffffffL / C::kThreads - total) return hipErrorInvalidValue;
     p.tiles_m = (int)tm;
@@ -479,7 +484,7 @@ template <typename T> struct Block {
     const bool al = (((uintptr_t)P.x | (uintptr_t)P.w0 | (uintptr_t)P.w1) & 15) == 0 && P.ldx % kVec == 0 && P.ldw0 % kVec == 0 &&
                     P.ldw1 % kVec == 0 && P.K % kVec == 0;
     const dim3 grid((unsigned)((P.N + 15) / 16));
-#define BUTD_FEW_ROWS(MT, AL) hipLaunchKernelGGL((few_rows_kernel<T, PARTS, MT, AL, 8>), grid, dim3(512), 0, stream, P)
+#define BUTD_FEW_ROWS(MT, AL) hipLaunchKernelGGL((few_rows_kernel<T, PARTS, MT, AL>), grid, dim3(512), 0, stream, P)
     if (P.M <= 16) {
       if (al) BUTD_FEW_ROWS(1, true); else BUTD_FEW_ROWS(1, false);
     } else if (P.M <= 32) {
