@@ -251,7 +251,8 @@ template <typename T> __global__ __launch_bounds__(256) void column_sum_kernel(c
 }
 // ---- plan -----------------------------------------------------------------------------------------------------------------
 constexpr int kCUs = 256;
-constexpr long kMaxBlocks = 0xffffffffL / 256;       // a launch has to stay below 2^32 threads
+constexpr long kMaxThreads = 0xffffffffL;            // a launch has to stay below 2^32 threads
+constexpr long kMaxBlocks = kMaxThreads / 256;
 constexpr long kMaxLd = 1L << 22;      // bytes between rows: 256 rows of a tile stay within a buffer descriptor's 2 GB
 
 // what butd_gated_ffn_set_tile asks for, read once a call: a plan is counted and carried out with one setting.  0: the rule
@@ -314,6 +315,7 @@ template <typename T> inline TileChoice choose(Forced forced, const Shape *shape
       tiles += (double)((shapes[i].M + m.size - 1) / m.size) * (double)((shapes[i].N + m.size - 1) / m.size);
       elems += (double)shapes[i].M * (double)shapes[i].N;
     }
+    if (m.size < 256 && tiles * 256.0 > (double)kMaxThreads) continue;       // (only a larger tile's launch has room for them)
     for (int s : splits) {
       if (s > 1 && (!can_split || steps < 3L * s)) break;
       const double turn = (double)((steps + s - 1) / s) + m.fill, bytes = s == 1 ? epilogue_bytes : 4.0;
@@ -344,7 +346,8 @@ template <typename T> inline double few_rows_us(long M, long N, long K, int part
   return 3.0 + (all > one ? all : one);
 }
 
-template <class C> inline hipError_t launch_tiles(Launch &L, hipStream_t stream) {
+// run == false, here and below: only what would be refused
+template <class C> inline hipError_t launch_tiles(Launch &L, bool run, hipStream_t stream) {
   constexpr int nw = C::kind == kGateUp ? C::TN / 2 : C::TN, bk = Num<typename C::type>::kBK;
   long total = 0;
   int slices = 1;
@@ -356,7 +359,7 @@ template <class C> inline hipError_t launch_tiles(Launch &L, hipStream_t stream)
       if (p.pad < p.N || (p.pad | p.ldc | p.ldaux) & 3 || at & 15) return hipErrorInvalidValue;
     }
     const long tm = ((long)p.M + C::TM - 1) / C::TM, tn = ((long)p.N + nw - 1) / nw;
-    if (tm * tn > 0xffffffffL / C::kThreads - total) return hipErrorInvalidValue;
+    if (tm * tn > kMaxThreads / C::kThreads - total) return hipErrorInvalidValue;
     p.tiles_m = (int)tm;
     p.tiles_n = (int)tn;
     p.first = (int)total;
@@ -367,6 +370,7 @@ template <class C> inline hipError_t launch_tiles(Launch &L, hipStream_t stream)
     if (p.split > slices) slices = p.split;
   }
   L.total = (int)total;
+  if (!run) return hipSuccess;
   hipLaunchKernelGGL((tile_kernel<C>), dim3((unsigned)total, (unsigned)slices), dim3(C::kThreads), 0, stream, L);
   return hipGetLastError();
 }
@@ -380,14 +384,14 @@ template <class C> inline hipError_t launch_tiles(Launch &L, hipStream_t stream)
   template __global__ void tile_kernel<Config<T, kGrad, true, false, TM, TM, WM, WN>>(const Launch);
 
 // The three tiles of every kind.  The smallest of kGateUp has its waves stacked along m: a wave holds both parts of its columns.
-template <typename T, int KIND, Layout LAY> inline hipError_t run_tiles(Launch &L, int size, hipStream_t stream) {
+template <typename T, int KIND, Layout LAY> inline hipError_t run_tiles(Launch &L, int size, bool run, hipStream_t stream) {
   constexpr bool ak = LAY != kTN, bk = LAY == kNT;
   if constexpr (sizeof(T) == 2) {
-    if (size == 256) return launch_tiles<Config<T, KIND, ak, bk, 256, 256, 2, 4>>(L, stream);
+    if (size == 256) return launch_tiles<Config<T, KIND, ak, bk, 256, 256, 2, 4>>(L, run, stream);
   }
-  if (size == 128) return launch_tiles<Config<T, KIND, ak, bk, 128, 128, 2, 2>>(L, stream);
-  if constexpr (KIND == kGateUp) return launch_tiles<Config<T, KIND, ak, bk, 64, 64, 4, 1>>(L, stream);
-  else return launch_tiles<Config<T, KIND, ak, bk, 64, 64, 2, 2>>(L, stream);
+  if (size == 128) return launch_tiles<Config<T, KIND, ak, bk, 128, 128, 2, 2>>(L, run, stream);
+  if constexpr (KIND == kGateUp) return launch_tiles<Config<T, KIND, ak, bk, 64, 64, 4, 1>>(L, run, stream);
+  else return launch_tiles<Config<T, KIND, ak, bk, 64, 64, 2, 2>>(L, run, stream);
 }
 
 template <typename T> struct Block {
@@ -417,9 +421,10 @@ template <typename T> struct Block {
     Operand take(const void *p, long ld, long rows, int cols) {
       return direct(p, ld, cols) ? Operand{p, ld} : pack(p, ld, rows, cols);
     }
-    hipError_t run(hipStream_t stream) {
+    hipError_t launch(bool run, hipStream_t stream) {
       if (!L.count) return hipSuccess;
       if (blocks > kMaxBlocks) return hipErrorInvalidValue;
+      if (!run) return hipSuccess;
       hipLaunchKernelGGL((copy_rows_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, L);
       return hipGetLastError();
     }
@@ -456,16 +461,17 @@ template <typename T> struct Block {
       if (p.split > 1) add_fold(F, p.slab, p.slab_stride, slab_ld(p.N), p.split, p.M, p.N, p.c, p.ldc, p.bias0);
     }
   }
-  static hipError_t run_folds(const Folds &F, hipStream_t stream) {
+  static hipError_t run_folds(const Folds &F, bool run, hipStream_t stream) {
     if (!F.count) return hipSuccess;
     if (F.blocks > kMaxBlocks) return hipErrorInvalidValue;
+    if (!run) return hipSuccess;
     hipLaunchKernelGGL((fold_kernel<T>), dim3((unsigned)F.blocks), dim3(256), 0, stream, F);
     return hipGetLastError();
   }
-  static hipError_t fold(const Launch &L, hipStream_t stream) {
+  static hipError_t fold(const Launch &L, bool run, hipStream_t stream) {
     Folds F{};
     add_folds(F, L);
-    return run_folds(F, stream);
+    return run_folds(F, run, stream);
   }
   static void slabs(Launch &L, int split, Arena &ws) {
     for (int i = 0; i < L.count; ++i) {
@@ -480,7 +486,8 @@ template <typename T> struct Block {
     }
   }
 
-  template <int PARTS> static hipError_t few_rows(const FewRows &P, hipStream_t stream) {
+  template <int PARTS> static hipError_t few_rows(const FewRows &P, bool run, hipStream_t stream) {
+    if (!run) return hipSuccess;
     const bool al = (((uintptr_t)P.x | (uintptr_t)P.w0 | (uintptr_t)P.w1) & 15) == 0 && P.ldx % kVec == 0 && P.ldw0 % kVec == 0 &&
                     P.ldw1 % kVec == 0 && P.K % kVec == 0;
     const dim3 grid((unsigned)((P.N + 15) / 16));
@@ -496,7 +503,7 @@ template <typename T> struct Block {
     return hipGetLastError();
   }
 
-  // run == false: only count the workspace
+  // run == false: count the workspace and refuse what a launch cannot hold; nothing is launched
   static hipError_t forward(const butd_gated_ffn_args &A, Arena &ws, bool run, hipStream_t stream) {
     const int M = (int)A.rows, E = A.width, F = A.hidden;
     if (M == 0) return hipSuccess;
@@ -535,23 +542,22 @@ template <typename T> struct Block {
       d.c = A.y; d.ldc = A.ld_y; d.bias0 = A.b_down;
       slabs(D, dc.split, ws);
     }
-    if (!run) return hipSuccess;
-    if ((err = pk.run(stream)) != hipSuccess) return err;
+    if ((err = pk.launch(run, stream)) != hipSuccess) return err;
     if (stream_in) {
       FewRows P{A.x, A.w_gate, A.w_up, A.ld_x, A.ld_gate, A.ld_up, M, F, E, A.activation, A.h, A.ld_h, (int)A.ld_h,
                 A.b_gate, A.b_up, A.a, A.b, A.ld_h};
-      err = few_rows<2>(P, stream);
+      err = few_rows<2>(P, run, stream);
     } else {
-      err = run_tiles<T, kGateUp, kNT>(G, gc.size, stream);
+      err = run_tiles<T, kGateUp, kNT>(G, gc.size, run, stream);
     }
     if (err != hipSuccess) return err;
     if (stream_out) {
       FewRows P{A.h, A.w_down, A.w_down, A.ld_h, A.ld_down, A.ld_down, M, E, F, A.activation, A.y, A.ld_y, 0,
                 A.b_down, nullptr, nullptr, nullptr, 0};
-      return few_rows<1>(P, stream);
+      return few_rows<1>(P, run, stream);
     }
-    if ((err = run_tiles<T, kPlain, kNT>(D, dc.size, stream)) != hipSuccess) return err;
-    return fold(D, stream);
+    if ((err = run_tiles<T, kPlain, kNT>(D, dc.size, run, stream)) != hipSuccess) return err;
+    return fold(D, run, stream);
   }
 
   static hipError_t backward(const butd_gated_ffn_args &A, Arena &ws, bool run, hipStream_t stream) {
@@ -639,21 +645,20 @@ template <typename T> struct Block {
       c.part = (float *)ws.take((long)c.chunks * c.cols * 4);
       if (c.chunks > chunks) chunks = c.chunks;
     }
-    if (!run) return hipSuccess;
-    if ((err = pk.run(stream)) != hipSuccess) return err;
-    if (inner && (err = run_tiles<T, kGrad, kNN>(G, gc.size, stream)) != hipSuccess) return err;
-    if (S.count) {
+    if ((err = pk.launch(run, stream)) != hipSuccess) return err;
+    if (inner && (err = run_tiles<T, kGrad, kNN>(G, gc.size, run, stream)) != hipSuccess) return err;
+    if (S.count && run) {
       hipLaunchKernelGGL((column_sum_kernel<T>), dim3((unsigned)blocks, (unsigned)chunks), dim3(256), 0, stream, S);
       if ((err = hipGetLastError()) != hipSuccess) return err;
     }
-    if (A.dx && (err = run_tiles<T, kPlain, kNN>(X, xc.size, stream)) != hipSuccess) return err;
-    if (W.count && (err = run_tiles<T, kPlain, kTN>(W, wc.size, stream)) != hipSuccess) return err;
+    if (A.dx && (err = run_tiles<T, kPlain, kNN>(X, xc.size, run, stream)) != hipSuccess) return err;
+    if (W.count && (err = run_tiles<T, kPlain, kTN>(W, wc.size, run, stream)) != hipSuccess) return err;
     // the slabs of dx and of the weight gradients and the bias gradients' row chunks in one launch
     Folds last{};
     add_folds(last, X);
     add_folds(last, W);
     for (int i = 0; i < S.count; ++i) add_fold(last, S.c[i].part, S.c[i].cols, S.c[i].cols, S.c[i].chunks, 1, S.c[i].cols, S.c[i].out, S.c[i].cols, nullptr);
-    return run_folds(last, stream);
+    return run_folds(last, run, stream);
   }
 };
 

@@ -18,7 +18,7 @@ ffn::Forced forced() {
   return ffn::Forced{v & 1023, v >> 10};
 }
 
-constexpr long kMostRows = 1L << 27;     // (a launch of the smallest tiles stays below 2^32 threads)
+constexpr long kMostRows = 1L << 27;     // (rows and products of them by 16 bytes a row fit the plan's integers)
 
 bool valid(const butd_gated_ffn_args *a, bool backward) {
   if (!a || a->dtype < BUTD_FFN_F32 || a->dtype > BUTD_FFN_F16) return false;

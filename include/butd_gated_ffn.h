@@ -72,7 +72,9 @@ long butd_gated_ffn_ld_hidden(int dtype, int hidden);
 int butd_gated_ffn_set_tile(int tile, int split);
 
 /* Bytes of device scratch (16-byte aligned) that the call with these arguments needs: a function of dtype, sizes, strides,
- * of the pointers' alignment and of which of them are NULL.  Negative: the arguments are refused (-hipErrorInvalidValue). */
+ * of the pointers' alignment and of which of them are NULL.  Negative: the arguments are refused (-hipErrorInvalidValue), by the
+ * call too and before it launches anything -- also where a launch would have 2^32 threads or more: copies of operands (of above
+ * 2^32 16-byte pieces), tiles that the hook forces. */
 long butd_gated_ffn_fwd_workspace(const butd_gated_ffn_args *args);
 long butd_gated_ffn_bwd_workspace(const butd_gated_ffn_args *args);
 

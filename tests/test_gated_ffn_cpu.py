@@ -163,3 +163,39 @@ def test_a_plan_is_made_of_one_setting_of_the_tuning_hook():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     out = subprocess.run([sys.executable, "-c", _HOOK_WHILE_PLANNING.format(root=root)], capture_output=True, text=True, timeout=120)
     assert out.returncode == 0, (out.returncode, out.stderr[-1000:])
+
+
+def test_what_a_launch_cannot_hold_is_refused_by_the_query():
+    """2^27 rows: the rule takes tiles whose launch has room for them; the smallest tiles, forced, and copies of odd rows are
+    refused by the workspace query as by the call, which launches nothing."""
+    from butd_detr_amd import _hiplib
+    lib = _hiplib.load()
+    invalid = 1                                                            # hipErrorInvalidValue
+
+    def refused(backward, **kw):
+        a = _filled(lib, rows=1 << 27, **kw)
+        if backward:
+            a.a, a.b, a.dy, a.dx, a.ld_dy, a.ld_dx, a.dw_gate = 4096, 8192, 12288, 16384, kw["width"], kw["width"], 4096
+        query, call = ((lib.butd_gated_ffn_bwd_workspace, lib.butd_gated_ffn_bwd) if backward
+                       else (lib.butd_gated_ffn_fwd_workspace, lib.butd_gated_ffn_fwd))
+        need = query(ctypes.byref(a))
+        assert need >= 0 or need == -invalid
+        if need < 0:
+            assert call(ctypes.byref(a), 4096, 1 << 62, None) == invalid   # (a call that is accepted would launch: not made)
+        return need < 0
+    for dtype in (0, 1, 2):
+        for backward in (False, True):
+            for width, hidden in ((16, 512), (16, 4096), (512, 16), (768, 256)):
+                # the largest tile: 128 rows x 64 columns of h (128 of the other products) on 256 threads, fp32; twice each, 16 bits
+                n = 1 if dtype == 0 else 2
+                columns = max(-(-hidden // ((128 if backward else 64) * n)), -(-width // (128 * n)))
+                threads = (1 << 27) // (128 * n) * columns * 256 * n
+                assert refused(backward, dtype=dtype, width=width, hidden=hidden) == (threads >= 1 << 32), (dtype, backward, width, hidden)
+            assert refused(backward, dtype=dtype, width=777, hidden=256), (dtype, backward)
+    lib.butd_gated_ffn_set_tile(64, 1)
+    try:
+        for backward in (False, True):
+            assert refused(backward, width=16, hidden=1024)
+            assert not refused(backward, width=16, hidden=24)
+    finally:
+        lib.butd_gated_ffn_set_tile(0, 0)
