@@ -25,11 +25,7 @@ COMMON = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-I" + INCLUDE,
           "-Wall", "-Wno-unused-function"]
 # No packed fp32 arithmetic (v_pk_add / mul / fma_f32), which hipcc -O3 forms by itself from ordinary float code: some of its
 # forms have given wrong results on this part now and then.  (The host pass does not know the feature and says so: harmless.)
-# One unit keeps the instructions it was tuned and tested with: in sa_ops.hip packing also decides which products are fused
-# with their sums, and the set-abstraction parity tests count the max-pool winners that change when those roundings do --
-# without packing 2 of 128 winners move and the mean error of a bias gradient is 1.3e-4 where the tests allow 1e-4.
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-PACKED_UNITS = ("sa_ops.hip",)
 # Per-TU flags.  The index kernels must round exactly like the oracle: no FMA contraction.
 # Wave priority of the MAIN queue's kernels (s_setprio at kernel entry; every unit but the index ops the prefetch branch
 # runs): the captured step's prefetch branches -- the next batch's furthest-point sampling on 8 CUs for 3.4 ms, its
@@ -84,7 +80,7 @@ def _tu_flags(name):
     flags = TU_FLAGS.get(name, [])
     if "-mllvm" in flags and not _supported(flags):
         flags = []
-    return flags + (MAIN_PRIO if name in MAIN_UNITS else []) + ([] if name in PACKED_UNITS else NO_PACKED_F32)
+    return flags + (MAIN_PRIO if name in MAIN_UNITS else []) + NO_PACKED_F32
 
 
 def _sources():

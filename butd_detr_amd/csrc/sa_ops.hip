@@ -25,6 +25,18 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Which products are fused with their sums is written down here, not left to the vectoriser: the max-pool winners of set
+// abstraction and the BatchNorm statistics depend on the last bit of Z and of the sums, and the parity tests count winners.
+// rounded(): a product that is rounded before it is added.  add_product(): of a thread's four columns 0 and 1 take one
+// rounding (fused), 2 and 3 two -- what the unit computed when its arithmetic was packed in pairs, bit for bit.
+__device__ inline float rounded(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+__device__ inline float add_product(int column, float a, float b, float sum) {
+  return column < 2 ? __builtin_fmaf(a, b, sum) : sum + rounded(a, b);
+}
+
 // ---------------------------------------------------------------------------------------- grouping
 __global__ __launch_bounds__(kThreads) void sa_group_kernel(int N, int np, int ns, int C,
                                                             const float *__restrict__ xyz,
@@ -102,7 +114,7 @@ __global__ __launch_bounds__(kThreads) void sa_colstats_kernel(
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[e] += v[e];
-          q[e] += v[e] * v[e];
+          q[e] = add_product(e, v[e], v[e], q[e]);
         }
       }
     }
@@ -112,7 +124,7 @@ __global__ __launch_bounds__(kThreads) void sa_colstats_kernel(
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[e] += v[e];
-        q[e] += v[e] * v[e];
+        q[e] = __builtin_fmaf(v[e], v[e], q[e]);
       }
     }
   }
@@ -132,7 +144,7 @@ __global__ __launch_bounds__(kThreads) void sa_colstats_kernel(
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[e] += v[e];
-          q[e] += v[e] * v[e];
+          q[e] = add_product(e, v[e], v[e], q[e]);
           if (v[e] > mx[e]) { mx[e] = v[e]; ax[e] = k; }
           if (v[e] < mn[e]) { mn[e] = v[e]; an[e] = k; }
         }
@@ -194,10 +206,10 @@ __global__ __launch_bounds__(kThreads) void sa_thin_conv_kernel(
     for (int e = 0; e < 4; ++e) {
       float a = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) a += x[k] * w[e][k];
+      for (int k = 0; k < 8; ++k) a = add_product(e, x[k], w[e][k], a);
       z[e] = a;
       s[e] += a;
-      q[e] += a * a;
+      q[e] = __builtin_fmaf(a, a, q[e]);
     }
     *reinterpret_cast<float4 *>(Z + (row0 + r) * C + cq * 4) = make_float4(z[0], z[1], z[2], z[3]);
   }
@@ -245,8 +257,8 @@ __global__ void sa_bn_finalize_kernel(int C, long count, const double *__restric
     mu = (float)m;
     var = (float)v;
     const double unbiased = count > 1 ? v * (double)count / (double)(count - 1) : v;
-    running_mean[c] = (1.f - momentum) * running_mean[c] + momentum * mu;
-    running_var[c] = (1.f - momentum) * running_var[c] + momentum * (float)unbiased;
+    running_mean[c] = rounded(1.f - momentum, running_mean[c]) + rounded(momentum, mu);
+    running_var[c] = rounded(1.f - momentum, running_var[c]) + rounded(momentum, (float)unbiased);
   } else {
     mu = running_mean[c];
     var = running_var[c];
@@ -301,7 +313,7 @@ __global__ __launch_bounds__(kThreads) void sa_pool_bwd_stats_kernel(
       if (sc * z + sh > 0.f) {
         const float dy = d_out_pm[g * C + col];
         s1 += dy;
-        s2 += dy * (z - mu) * rs;
+        s2 += rounded(dy * (z - mu), rs);
       }
     }
   }
@@ -391,7 +403,7 @@ __global__ __launch_bounds__(kThreads) void sa_mask_stats_kernel(
     for (int e = 0; e < 4; ++e) {
       if (!(sc[e] * z[e] + sh[e] > 0.f)) g[e] = 0.f;
       s1[e] += g[e];
-      s2[e] += g[e] * (z[e] - mu[e]) * rs[e];
+      s2[e] = __builtin_fmaf(g[e] * (z[e] - mu[e]), rs[e], s2[e]);
     }   // read-only pass: butd_sa_dz_mid re-derives the mask from Z instead of reading a stored g
   }
 #pragma unroll
