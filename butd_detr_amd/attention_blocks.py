@@ -17,6 +17,7 @@ import math
 
 import torch
 import torch.nn.functional as F
+from torch import nn
 
 _BACKEND = "torch"
 
@@ -152,17 +153,35 @@ def gated_ffn(ffn, x):
     return ffn.down(act(ffn.gate(x)) * ffn.up(x))
 
 
+def _wide_norm(norm, v):
+    """norm(v) for v in 32 bits or more and parameters of any type."""
+    weight, bias = (None if p is None else p.to(v.dtype) for p in (getattr(norm, "weight", None), getattr(norm, "bias", None)))
+    if isinstance(norm, nn.LayerNorm):
+        return F.layer_norm(v, norm.normalized_shape, weight, bias, norm.eps)
+    if isinstance(norm, nn.RMSNorm):
+        return F.rms_norm(v, norm.normalized_shape, weight, norm.eps)
+    return norm(v)
+
+
 def residual_norm(x, residual=None, *, post_norm=None, gate=None, residual_scale=1.0, pre_norm=None):
-    """(stream, normed): stream = residual_scale * residual + gate * post_norm(x), normed = pre_norm(stream) | None."""
+    """(stream, normed): stream = residual_scale * residual + gate * post_norm(x), normed = pre_norm(stream) | None.
+    Both backends compute in 32 bits (float64 tensors, torch backend only: in 64) from the tensors' values, take parameters of x's
+    type or float32, norm the unrounded stream and round each output once: the stream to the residual's type, normed to x's."""
     if _BACKEND == "hip" and x.is_cuda:
         from . import residual_norm as fused
         return fused.residual_norm(x, residual, post_norm=post_norm, gate=gate, residual_scale=residual_scale,
                                    pre_norm=pre_norm)
-    branch = x if post_norm is None else post_norm(x)
+    out = x.dtype if residual is None else residual.dtype
+    wide = torch.promote_types(torch.promote_types(x.dtype, out), torch.float32)
+    stream = x.to(wide)
+    if post_norm is not None:
+        stream = _wide_norm(post_norm, stream)
     if gate is not None:
-        branch = branch * (gate[:, None, :] if x.dim() == 3 and gate.dim() == 2 else gate)
-    stream = branch if residual is None else (residual_scale * residual + branch).to(residual.dtype)
-    return stream, None if pre_norm is None else pre_norm(stream).to(x.dtype)
+        stream = stream * (gate[:, None, :] if x.dim() == 3 and gate.dim() == 2 else gate).to(wide)
+    if residual is not None:
+        stream = residual_scale * residual.to(wide) + stream
+    normed = None if pre_norm is None else _wide_norm(pre_norm, stream).to(x.dtype)
+    return x if residual is None and gate is None and post_norm is None else stream.to(out), normed
 
 
 def gated_ffn_block(ffn, x, *, pre_norm=None, normed=None, post_norm=None, gate=None, residual_scale=1.0, next_norm=None):

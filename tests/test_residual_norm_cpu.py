@@ -114,3 +114,32 @@ def test_default_epsilon_is_the_module_s_own(dtype, params):
     want = 2.0 ** -12 / (2.0 ** -24 + eps) ** 0.5
     assert abs(y - want) <= want * (torch.finfo(dtype).eps / 2 + 2.0 ** -20), (y, want, eps)
     assert _norm("pre_norm", nn.RMSNorm(64, eps=0.5), 64)[3] == 0.5
+
+
+@pytest.mark.parametrize("x_type, stream_type", [(torch.bfloat16, torch.float32), (torch.bfloat16, torch.bfloat16),
+                                                 (torch.float16, torch.float32), (torch.float32, torch.float32)])
+@pytest.mark.parametrize("params", [None, torch.float32])
+@pytest.mark.parametrize("kind", [nn.LayerNorm, nn.RMSNorm])
+def test_torch_backend_takes_and_rounds_what_the_kernels_do(kind, params, x_type, stream_type):
+    """Parameters of x's type or float32 beside a stream of either type; one rounding an output, normed from the unrounded
+    stream.  Inside 32 bits: 2^-18 of the largest term covers the row's sums."""
+    from butd_detr_amd import attention_blocks as ab
+    torch.manual_seed(2)
+    cols = 48
+    x, r = torch.randn(3, 4, cols).to(x_type), (4 * torch.randn(3, 4, cols)).to(stream_type)
+    post, pre = kind(cols).to(params or x_type), kind(cols).to(params or x_type)
+    gate = torch.rand(3, cols).to(x_type)
+    prev = ab.get_backend()
+    try:
+        ab.set_backend("torch")
+        stream, normed = ab.residual_norm(x, r, post_norm=post, gate=gate, residual_scale=0.75, pre_norm=pre)
+        alone = ab.residual_norm(x, post_norm=post)
+        assert ab.residual_norm(x, pre_norm=pre)[0] is x
+    finally:
+        ab.set_backend(prev)
+    n1, n2 = (kind(cols, eps=m.eps if m.eps is not None else 2.0 ** -23).double() for m in (post, pre))
+    s = 0.75 * r.double() + gate.double()[:, None] * n1(x.double())
+    assert stream.dtype == stream_type and normed.dtype == x_type and alone[0].dtype == x_type and alone[1] is None
+    for got, want in ((stream, s), (normed, n2(s)), (alone[0], n1(x.double()))):
+        u = torch.finfo(got.dtype).eps / 2
+        assert float(((got.double() - want).abs() - u * want.abs() - 2.0 ** -18 * (1 + u) * 16).max()) <= 0
