@@ -188,11 +188,11 @@ def gated_ffn_block(ffn, x, *, pre_norm=None, normed=None, post_norm=None, gate=
     """The pre-norm / sandwich-norm feed-forward block of a layer stack:
         stream = residual_scale * x + gate * post_norm(FFN(pre_norm(x))),   FFN = gated_ffn(ffn, .)
     -> (stream, next_norm(stream) | None).  ``next_norm``: the norm in front of the NEXT block, computed by the kernel that
-    writes the stream; that block then takes it as ``normed`` in place of ``pre_norm`` (a float32 stream around a 16-bit FFN
-    needs it: pre_norm alone would return the stream's type)."""
+    writes the stream; that block then takes it as ``normed`` in place of ``pre_norm``.  A stack begins with ``pre_norm``: in front
+    of a 16-bit FFN the normed float32 stream is rounded to the FFN's type, by one more pass over it."""
     if (pre_norm is None) == (normed is None):
         raise ValueError("gated_ffn_block: one of pre_norm and normed")
     if normed is None:
-        normed = residual_norm(x, pre_norm=pre_norm)[1]
+        normed = residual_norm(x, pre_norm=pre_norm)[1].to(ffn.gate.weight.dtype)
     return residual_norm(gated_ffn(ffn, normed), x, post_norm=post_norm, gate=gate, residual_scale=residual_scale,
                          pre_norm=next_norm)

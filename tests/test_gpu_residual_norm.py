@@ -479,3 +479,100 @@ def test_layer_norm_of_a_constant_row_is_zero(dtype):
     from butd_detr_amd.residual_norm import residual_norm
     x = torch.full((2, 40), 3.0, device="cuda", dtype=dtype)
     assert float(residual_norm(x, pre_norm=nn.LayerNorm(40, device="cuda", dtype=dtype))[1].abs().max()) == 0.0
+
+
+class _Rounded(torch.autograd.Function):
+    """rounds to ``dtype`` what goes forward and / or what comes back, values held in 64 bits; ``noise``: each value is moved by
+    that much of the tensor's root mean square (normally distributed) before"""
+
+    @staticmethod
+    def _round(v, dtype, noise):
+        if noise:
+            v = v + noise * v.square().mean().sqrt() * torch.randn(v.shape, device=v.device, dtype=v.dtype)
+        return v.to(dtype).double()
+
+    @staticmethod
+    def forward(ctx, v, dtype, forth, back, noise):
+        ctx.dtype, ctx.back, ctx.noise = dtype, back, noise
+        return _Rounded._round(v, dtype, noise) if forth else v.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        return (_Rounded._round(g, ctx.dtype, ctx.noise) if ctx.back else g), None, None, None, None
+
+
+def _unit(m, v):
+    if m["bias"] is not None:
+        v = v - v.mean(-1, keepdim=True)
+    v = v * ((v * v).mean(-1, keepdim=True) + m["eps"]).rsqrt() * m["weight"]
+    return v if m["bias"] is None else v + m["bias"]
+
+
+def _emulated_stack(leaves, norms, dtype, d_out, noise=0.0):
+    """Two sandwich blocks in 64 bits, rounded where the kernels round: normed, h and y forward; the gradients of h's two factors,
+    of the FFN's input and output and of each use of the gate backward; every output.  -> outputs and gradients"""
+    both, forth, back = (lambda v, f=f, b=b: _Rounded.apply(v, dtype, f, b, noise) for f, b in ((True, True), (True, False), (False, True)))
+    leaves = [t.detach().double().requires_grad_(True) for t in leaves]
+    x, gate, weights = leaves[0], leaves[1], leaves[2:]
+    stream, normed = x, both(_unit(norms[0], x))
+    for i, scale in enumerate((1.0, 0.7)):
+        w_gate, w_up, w_down = weights[3 * i:3 * i + 3]
+        a, b = back(normed @ w_gate.t()), back(normed @ w_up.t())
+        v = a * torch.sigmoid(a) if i == 0 else 0.5 * a * torch.erfc(-a * 0.5 ** 0.5)
+        y = both(forth(v * b) @ w_down.t())
+        stream = scale * stream + back(gate)[:, None] * _unit(norms[2 * i + 1], y)
+        normed = both(_unit(norms[2 * i + 2], stream))
+    out = [stream, normed]
+    out += torch.autograd.grad(out, leaves, [p.double() for p in d_out])
+    wide = lambda i: i in (0, 2)                             # (the stream and x are 32 bits)       # noqa: E731
+    return [t.detach() if wide(i) else _Rounded._round(t.detach(), dtype, noise) for i, t in enumerate(out)]
+
+
+def stack_inputs(rows, dtype, device="cuda"):
+    from butd_detr_amd.gated_ffn import GatedFeedForward
+    torch.manual_seed(6)
+    cols, hidden = 288, 512
+    ffns = [GatedFeedForward(cols, hidden, a).to(device, dtype) for a in ("silu", "gelu")]
+    norms = [norm_of(k, cols, torch.float32).to(device) for k in ("rms", "layer", "rms", "rms", "layer")]
+    gate = torch.rand(rows[0], cols).to(device, dtype)
+    x, p_stream, p_normed = (torch.randn(*rows, cols).to(device) for _ in range(3))
+    leaves = [x.requires_grad_(True), gate.requires_grad_(True)] + [q for f in ffns for q in f.parameters()]
+    n64 = [dict(weight=m.weight.detach().double(), bias=None if getattr(m, "bias", None) is None else m.bias.detach().double(), eps=m.eps)
+           for m in norms]
+    return ffns, norms, leaves, [p_stream, p_normed.to(dtype)], n64
+
+
+def far(got, want):
+    return [float((g.double() - w.double()).norm() / w.double().norm()) for g, w in zip(got, want)]
+
+
+def stack_limits(leaves, n64, dtype, d_out):
+    """How far an emulation goes whose every value is moved by a 32-bit computation's error before it is rounded.  A sum of n
+    products in 32 bits rounds n times, each time a sum that has grown to sqrt(k) of its terms' size by 2^-24 of it at most, 0.4
+    of that in the root mean square: 0.4 2^-24 sqrt(1 + 2 + ... + n) in all, 0.28 sqrt(n) 2^-24 of the result -- 2^-21.2 for the
+    up to 600 products here, taken as 2^-21.  Moved values round the other way here and there, and that goes on through the
+    later blocks: the distance of the two emulations, taken twice for the chance in it, is what the kernels may be off by; 2^-19
+    for what is not rounded."""
+    want = _emulated_stack(leaves, n64, dtype, d_out)
+    return want, [2 * v + 2.0 ** -19 for v in far(_emulated_stack(leaves, n64, dtype, d_out, noise=2.0 ** -21), want)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [(1, 1), (2, 9), (2, 300)])
+def test_a_stack_of_gated_blocks_rounds_where_the_kernels_do(rows, dtype):
+    """The stack of test_a_stack_of_gated_blocks, begun by ``pre_norm``, against 64 bits with the same roundings."""
+    from butd_detr_amd import attention_blocks as ab
+    ffns, norms, leaves, d_out, n64 = stack_inputs(rows, dtype)
+    prev = ab.get_backend()
+    try:
+        ab.set_backend("hip")
+        stream, normed = ab.gated_ffn_block(ffns[0], leaves[0], pre_norm=norms[0], post_norm=norms[1], gate=leaves[1], next_norm=norms[2])
+        assert normed.dtype == dtype
+        out = ab.gated_ffn_block(ffns[1], stream, normed=normed, post_norm=norms[3], gate=leaves[1], residual_scale=0.7,
+                                 next_norm=norms[4])
+        got = [t.detach() for t in out + torch.autograd.grad(out, leaves, d_out)]
+    finally:
+        ab.set_backend(prev)
+    want, limits = stack_limits(leaves, n64, dtype, d_out)
+    for i, (g, off, limit) in enumerate(zip(got, far(got, want), limits)):
+        assert g.dtype == (torch.float32 if i in (0, 2) else dtype) and off <= limit, (rows, dtype, i, off, limit)

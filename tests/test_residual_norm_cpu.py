@@ -143,3 +143,20 @@ def test_torch_backend_takes_and_rounds_what_the_kernels_do(kind, params, x_type
     for got, want in ((stream, s), (normed, n2(s)), (alone[0], n1(x.double()))):
         u = torch.finfo(got.dtype).eps / 2
         assert float(((got.double() - want).abs() - u * want.abs() - 2.0 ** -18 * (1 + u) * 16).max()) <= 0
+
+
+def test_a_block_begins_a_stack_of_16_bit_blocks_on_a_32_bit_stream():
+    from butd_detr_amd import attention_blocks as ab
+    from butd_detr_amd.gated_ffn import GatedFeedForward
+    torch.manual_seed(5)
+    ffn, norm = GatedFeedForward(16, 24, "silu").bfloat16(), nn.RMSNorm(16)
+    x = torch.randn(2, 3, 16)
+    prev = ab.get_backend()
+    try:
+        ab.set_backend("torch")
+        stream, normed = ab.gated_ffn_block(ffn, x, pre_norm=norm, next_norm=norm)
+        by_hand = ab.gated_ffn_block(ffn, x, normed=norm(x).bfloat16(), next_norm=norm)
+    finally:
+        ab.set_backend(prev)
+    assert stream.dtype == torch.float32 and normed.dtype == torch.bfloat16
+    assert torch.equal(stream, by_hand[0]) and torch.equal(normed, by_hand[1])
