@@ -2,6 +2,7 @@
 // allocation and the autograd nodes of butd_detr_amd.gated_ffn and butd_detr_amd.residual_norm in C++.  A small layer's pass
 // is bound by the host: as Python autograd functions over ctypes a forward + backward took about 145 us of it, the kernels
 // of 2048 rows x 288 take 25.
+#include <ATen/autocast_mode.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/hip/HIPStream.h>
@@ -188,8 +189,9 @@ struct GatedFfnNode : torch::autograd::Function<GatedFfnNode> {
   }
 };
 
-Tensor gated_ffn(const Tensor &x, const Tensor &w_gate, const Tensor &w_up, const Tensor &w_down, const Maybe &b_gate,
-                 const Maybe &b_up, const Maybe &b_down, int64_t activation) {
+// (grad: of the call's own tensors, where gated_ffn has looked at them already)
+Tensor gated_ffn_of(const Tensor &x, const Tensor &w_gate, const Tensor &w_up, const Tensor &w_down, const Maybe &b_gate,
+                    const Maybe &b_up, const Maybe &b_down, int64_t activation, std::optional<bool> grad) {
   TORCH_CHECK(x.dim() >= 1 && w_gate.dim() == 2, "gated_ffn: x must be (..., width) and w_gate (hidden, width)");
   const int64_t hidden = w_gate.size(0), width = w_gate.size(1);
   TORCH_CHECK(width >= 1 && hidden >= 1, "gated_ffn: width and hidden must be at least 1");
@@ -210,11 +212,24 @@ Tensor gated_ffn(const Tensor &x, const Tensor &w_gate, const Tensor &w_up, cons
   TORCH_CHECK(x.is_cuda(), "CPU not supported");
   TORCH_CHECK(x.numel() / width <= 1L << 27, "gated_ffn: at most 2^27 rows");
   const Tensor bg = value(b_gate), bu = value(b_up), bd = value(b_down);
-  if (wants_grad({x, w_gate, w_up, w_down, bg, bu, bd}, "gated_ffn"))
+  if (grad.has_value() ? *grad : wants_grad({x, w_gate, w_up, w_down, bg, bu, bd}, "gated_ffn"))
     return GatedFfnNode::apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation);
   return ffn_forward(rows_of(x), rows_of(w_gate), rows_of(w_up), rows_of(w_down), contiguous(bg), contiguous(bu), contiguous(bd),
                      activation, false)
       .y.view(x.sizes());
+}
+
+Tensor gated_ffn(const Tensor &x, const Tensor &w_gate, const Tensor &w_up, const Tensor &w_down, const Maybe &b_gate,
+                 const Maybe &b_up, const Maybe &b_down, int64_t activation) {
+  if (!x.is_cuda() || !at::autocast::is_autocast_enabled(at::kCUDA))
+    return gated_ffn_of(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation, std::nullopt);
+  // under autocast every operand goes to the type that linear layers take there
+  const at::ScalarType type = at::autocast::get_autocast_dtype(at::kCUDA);
+  const auto cast = [&](const Tensor &t) { return t.is_cuda() && dtype_of(t.scalar_type()) >= 0 ? t.to(type) : t; };
+  const auto cast_maybe = [&](const Maybe &t) { return t.has_value() ? Maybe(cast(*t)) : t; };
+  const bool grad = wants_grad({x, w_gate, w_up, w_down, value(b_gate), value(b_up), value(b_down)}, "gated_ffn");
+  return gated_ffn_of(cast(x), cast(w_gate), cast(w_up), cast(w_down), cast_maybe(b_gate), cast_maybe(b_up), cast_maybe(b_down),
+                      activation, grad);
 }
 
 // ---- norms around a block ---------------------------------------------------------------------------------------------------

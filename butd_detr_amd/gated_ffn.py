@@ -23,6 +23,7 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, acti
     one dtype (float32, bfloat16, float16) on one GPU.  ``activation``: silu, gelu (erf), gelu_tanh, relu or sigmoid.  Any
     sizes from 1 on and any number of rows, none included; rows may be strided (a slice of a wider buffer).  Widths or strides
     that are no multiple of 16 bytes cost a copy of that operand into padded rows, except for up to 64 rows in the forward pass.
+    Under autocast all tensors are cast to its type first, as for ``F.linear``.
     Runs on the current stream, also under graph capture; first derivatives only.  RuntimeError on CPU tensors and on shapes or
     types that do not fit."""
     kind = ACTIVATIONS.get(activation)

@@ -493,3 +493,50 @@ def test_the_documented_roundings_and_no_others(size, dtype):
         for k in want:
             far = float((got[k].double() - want[k].double()).norm() / want[k].double().norm())
             assert far <= limit, (size, kind, k, far / u, limit / u)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [5, 130])
+def test_autocast_casts_like_a_linear_layer(rows, kind):
+    """float32 parameters, x of either type: the call on cast tensors, gradients in the types the leaves have."""
+    from butd_detr_amd import attention_blocks as ab
+    from butd_detr_amd.gated_ffn import GatedFeedForward
+    t, dy = inputs(rows, 40, 56, torch.float32)
+    dy = dy.to(kind)
+    want = run({k: v.to(kind) for k, v in t.items()}, dy, "silu")
+    for x_type in (torch.float32, kind):
+        leaves = {k: v.to(x_type if k == "x" else torch.float32).requires_grad_(True) for k, v in t.items()}
+        with torch.autocast("cuda", kind):
+            y = _apply(leaves, "silu")
+            with torch.no_grad():
+                quiet = _apply(leaves, "silu")
+        assert y.dtype == kind and torch.equal(y, want["y"]) and torch.equal(quiet, y)
+        for (k, v), g in zip(leaves.items(), torch.autograd.grad(y, list(leaves.values()), dy)):
+            assert g.dtype == v.dtype and torch.equal(g, want["d_" + k].to(v.dtype)), k
+    torch.manual_seed(0)
+    ffn, x = GatedFeedForward(40, 56, bias=True).cuda(), t["x"].to(kind)
+    prev = ab.get_backend()
+    try:
+        for backend in ("torch", "hip"):
+            ab.set_backend(backend)
+            with torch.autocast("cuda", kind):
+                assert ffn(x).dtype == kind and ffn(x.float()).dtype == kind
+            with torch.autocast("cuda", kind, enabled=False):
+                assert ffn(x.float()).dtype == torch.float32
+    finally:
+        ab.set_backend(prev)
+    with torch.autocast("cuda", kind), pytest.raises(RuntimeError, match="not served"):
+        _apply({k: v.double() for k, v in t.items()}, "silu")
+
+
+def test_capture_beside_a_living_eager_graph_is_refused_under_autocast():
+    """the leaves are looked at, not their casts"""
+    t, _ = inputs(70, 48, 40, torch.float32)
+    leaves = {k: v.requires_grad_(True) for k, v in t.items()}
+    with torch.autocast("cuda", torch.bfloat16):
+        alive = _apply(leaves, "silu")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(RuntimeError, match="eager graph"):
+                _apply(leaves, "silu")
+    del alive
