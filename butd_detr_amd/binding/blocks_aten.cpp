@@ -5,8 +5,10 @@
 #include <ATen/autocast_mode.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <climits>
@@ -47,6 +49,13 @@ std::string python_shape(at::IntArrayRef s) {
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor value(const Maybe &t) { return t.has_value() ? *t : Tensor(); }
 Tensor contiguous(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
+
+// The kernels are no registered operators: a tracer would record the allocation of the outputs and nothing that fills them.
+void no_tracing(const char *what) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                  !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+              what, ": cannot be traced (torch.jit.trace, torch.fx make_fx)");
+}
 
 bool wants_grad(std::initializer_list<Tensor> ts, const char *what) {
   for (const Tensor &t : ts)
@@ -192,6 +201,7 @@ struct GatedFfnNode : torch::autograd::Function<GatedFfnNode> {
 // (grad: of the call's own tensors, where gated_ffn has looked at them already)
 Tensor gated_ffn_of(const Tensor &x, const Tensor &w_gate, const Tensor &w_up, const Tensor &w_down, const Maybe &b_gate,
                     const Maybe &b_up, const Maybe &b_down, int64_t activation, std::optional<bool> grad) {
+  no_tracing("gated_ffn");
   TORCH_CHECK(x.dim() >= 1 && w_gate.dim() == 2, "gated_ffn: x must be (..., width) and w_gate (hidden, width)");
   const int64_t hidden = w_gate.size(0), width = w_gate.size(1);
   TORCH_CHECK(width >= 1 && hidden >= 1, "gated_ffn: width and hidden must be at least 1");
@@ -356,6 +366,7 @@ struct ResidualNormNode : torch::autograd::Function<ResidualNormNode> {
 std::tuple<Maybe, Maybe> residual_norm(const Tensor &x, const Maybe &residual, const Maybe &gate, const Maybe &w1, const Maybe &b1,
                                        const Maybe &w2, const Maybe &b2, int64_t post_kind, int64_t pre_kind, double post_eps,
                                        double pre_eps, double scale) {
+  no_tracing("residual_norm");
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "residual_norm: x must be (..., cols) with cols >= 1");
   TORCH_CHECK(dtype_of(x.scalar_type()) >= 0, "residual_norm: ", x.scalar_type(), " is not served (float32, bfloat16, float16)");
   const int64_t cols = x.size(-1);

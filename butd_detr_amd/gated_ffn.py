@@ -24,8 +24,8 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, acti
     sizes from 1 on and any number of rows, none included; rows may be strided (a slice of a wider buffer).  Widths or strides
     that are no multiple of 16 bytes cost a copy of that operand into padded rows, except for up to 64 rows in the forward pass.
     Under autocast all tensors are cast to its type first, as for ``F.linear``.
-    Runs on the current stream, also under graph capture; first derivatives only.  RuntimeError on CPU tensors and on shapes or
-    types that do not fit."""
+    Runs on the current stream, also under graph capture; first derivatives only.  RuntimeError on CPU tensors, on shapes or
+    types that do not fit, under tracers (torch.jit.trace, make_fx), vmap and forward mode."""
     kind = ACTIVATIONS.get(activation)
     if kind is None:
         raise ValueError(f"gated_ffn: unknown activation {activation!r} (known: {', '.join(ACTIVATIONS)})")

@@ -37,10 +37,10 @@ def residual_norm(x, residual=None, *, post_norm=None, gate=None, residual_scale
     x (..., cols): a block's output, float32 / bfloat16 / float16, cols <= 8192; ``residual``: of x's shape and of x's dtype or
     float32 (the stream has its dtype; None counts as zeros, and without gate and post_norm too the stream IS x); ``post_norm``,
     ``pre_norm``: nn.LayerNorm / nn.RMSNorm over the last dimension (an ``eps`` of None is float32's, as the module takes it), or
-    None; ``gate``: (cols,), (batch, cols) for x (batch,
-    length, cols), or of x's shape.  Parameters of the norms and the gate have x's dtype or float32.  Computed in 32 bits, each
-    output rounded once; ``normed`` is the norm of the unrounded stream.  Runs on the current stream, also under graph capture;
-    first derivatives only.  RuntimeError on CPU tensors and on shapes or types that do not fit."""
+    None; ``gate``: (cols,), (batch, cols) for x (batch, length, cols), or of x's shape.  Parameters of the norms and the gate
+    have x's dtype or float32.  Computed in 32 bits, each output rounded once; ``normed`` is the norm of the unrounded stream.
+    Runs on the current stream, also under graph capture; first derivatives only.  RuntimeError on CPU tensors, on shapes or types that do not fit, under tracers (torch.jit.trace,
+    make_fx), vmap and forward mode."""
     cols = x.shape[-1] if x.dim() else 0
     w1, b1, post, post_eps = _norm("post_norm", post_norm, cols)
     w2, b2, pre, pre_eps = _norm("pre_norm", pre_norm, cols)

@@ -94,3 +94,18 @@ def test_a_library_with_another_argument_struct_is_refused(name, monkeypatch):
     monkeypatch.setattr(_hiplib, name, Longer)
     with pytest.raises(_hiplib.HipLibraryMissing, match="build it again"):
         _hiplib.load()
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("how", ["jit", "fx"])
+def test_tracing_is_refused(how):
+    """Neither block is a registered operator: a trace would hold the allocation of its output only."""
+    import torch
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from butd_detr_amd.gated_ffn import gated_ffn
+    from butd_detr_amd.residual_norm import residual_norm
+    w = torch.randn(12, 8)
+    trace = (lambda f, v: torch.jit.trace(f, (v,))) if how == "jit" else (lambda f, v: make_fx(f)(v))
+    for block in (lambda v: gated_ffn(v, w, w, w.t().contiguous()), lambda v: residual_norm(v, pre_norm=torch.nn.RMSNorm(8))[1]):
+        with torch.no_grad(), pytest.raises(RuntimeError, match="cannot be traced"):
+            trace(block, torch.randn(3, 8))

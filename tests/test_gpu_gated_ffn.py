@@ -540,3 +540,9 @@ def test_capture_beside_a_living_eager_graph_is_refused_under_autocast():
             with pytest.raises(RuntimeError, match="eager graph"):
                 _apply(leaves, "silu")
     del alive
+
+
+def test_vmap_is_refused():
+    t, _ = inputs(6, 8, 8, torch.float32, bias=False)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda v: _apply({**t, "x": v}, "silu"))(t["x"].view(2, 3, 8))

@@ -576,3 +576,9 @@ def test_a_stack_of_gated_blocks_rounds_where_the_kernels_do(rows, dtype):
     want, limits = stack_limits(leaves, n64, dtype, d_out)
     for i, (g, off, limit) in enumerate(zip(got, far(got, want), limits)):
         assert g.dtype == (torch.float32 if i in (0, 2) else dtype) and off <= limit, (rows, dtype, i, off, limit)
+
+
+def test_vmap_is_refused():
+    from butd_detr_amd.residual_norm import residual_norm
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda v: residual_norm(v, pre_norm=nn.RMSNorm(8, device="cuda"))[1])(torch.randn(2, 3, 8, device="cuda"))
