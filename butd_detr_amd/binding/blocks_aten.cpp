@@ -15,6 +15,7 @@
 #include <optional>
 #include <string>
 #include <tuple>
+#include <unordered_set>
 #include <vector>
 
 #include "butd_gated_ffn.h"
@@ -64,18 +65,29 @@ bool wants_grad(std::initializer_list<Tensor> ts, const char *what) {
   bool wanted = false;
   for (const Tensor &t : ts) wanted |= t.defined() && t.requires_grad();
   if (!wanted) return false;
-  // A leaf whose gradient accumulator an eager graph keeps alive belongs to that graph's stream.  A backward pass captured
-  // elsewhere makes that stream wait for the capture; the default stream cannot, which ends the process: refused here.
+  // A leaf whose gradient accumulator an eager graph keeps alive belongs to that graph's stream, as an eager graph's output
+  // does.  A backward pass captured elsewhere makes that stream wait for the capture; the default stream cannot, which ends the
+  // process: refused here, for the operands and for what stands behind views and casts of them that this capture has made.
   const hipStream_t stream = (hipStream_t)stream_of(*ts.begin());
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   if (!stream || hipStreamIsCapturing(stream, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return true;
-  for (const Tensor &t : ts) {
-    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
-    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
-    const auto owner = accumulator ? accumulator->stream() : std::nullopt;
-    TORCH_CHECK(!owner || c10::hip::HIPStreamMasqueradingAsCUDA(*owner).stream() != nullptr, what,
-                ": captured into a graph while an eager graph of the same leaves is alive on the default stream; release its "
-                "outputs first");
+  std::vector<std::shared_ptr<torch::autograd::Node>> open;
+  std::unordered_set<const torch::autograd::Node *> seen;
+  const auto visit = [&](const std::shared_ptr<torch::autograd::Node> &node) {
+    if (node && seen.insert(node.get()).second) open.push_back(node);
+  };
+  for (const Tensor &t : ts)
+    if (t.defined() && t.requires_grad()) visit(t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn());
+  while (!open.empty()) {
+    const auto node = open.back();
+    open.pop_back();
+    const auto s = node->stream();
+    if (!s || !s->device().is_cuda()) continue;
+    const hipStream_t owner = c10::hip::HIPStreamMasqueradingAsCUDA(*s).stream();
+    TORCH_CHECK(owner != nullptr, what, ": captured into a graph while an eager graph of the same leaves is alive on the default "
+                "stream; release its outputs first, or detach what is taken from it");
+    if (owner == stream)
+      for (const auto &edge : node->next_edges()) visit(edge.function);
   }
   return true;
 }

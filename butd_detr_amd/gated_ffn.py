@@ -21,8 +21,9 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, acti
 
     x (..., width); w_gate, w_up (hidden, width); w_down (width, hidden); biases (hidden), (hidden), (width) or None; all of
     one dtype (float32, bfloat16, float16) on one GPU.  ``activation``: silu, gelu (erf), gelu_tanh, relu or sigmoid.  Any
-    sizes from 1 on and any number of rows, none included; rows may be strided (a slice of a wider buffer).  Widths or strides
-    that are no multiple of 16 bytes cost a copy of that operand into padded rows, except for up to 64 rows in the forward pass.
+    sizes from 1 on and any number of rows, none included; rows of a matrix may be strided (a slice of a wider buffer; of more
+    dimensions such a slice is copied).  Widths or strides that are no multiple of 16 bytes cost a copy of that operand into
+    padded rows, except for up to 64 rows in the forward pass.
     Under autocast all tensors are cast to its type first, as for ``F.linear``.
     Runs on the current stream, also under graph capture; first derivatives only.  RuntimeError on CPU tensors, on shapes or
     types that do not fit, under tracers (torch.jit.trace, make_fx), vmap and forward mode."""

@@ -5,6 +5,7 @@ type (``eps / 2``), every value that is rounded to that type (h, da, db, the out
 products accumulated in 32 bits at most (n + 2) 2^-23 of the sum of their magnitudes; the activation and its slope, from
 hardware exponentials and reciprocals (each within 2^-22 of the value) on arguments whose own rounding enters through the
 exponential's slope, 2^-20 (1 + |a|).  Errors of a and b go through the slopes (|act''| <= 1.2 for all five)."""
+import gc
 import itertools
 
 import pytest
@@ -546,3 +547,34 @@ def test_vmap_is_refused():
     t, _ = inputs(6, 8, 8, torch.float32, bias=False)
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda v: _apply({**t, "x": v}, "silu"))(t["x"].view(2, 3, 8))
+
+
+def test_capture_beside_a_living_eager_graph_is_refused_for_casts_and_views():
+    """Operands that the capture casts or views: their leaves' gradients belong to the living graph all the same.  So does what
+    an eager graph hands over undetached.  (Only forward passes run here.)"""
+    t, dy = inputs(70, 40, 40, torch.float32)
+    leaves = {k: v.requires_grad_(True) for k, v in t.items()}
+    views = {"cast": lambda d: {k: v.bfloat16() for k, v in d.items()}, "view": lambda d: {**d, "w_up": d["w_up"].t().t()},
+             "sum": lambda d: {**d, "x": (d["x"] + 1) * 2}}
+    alive, between = _apply(leaves, "silu"), leaves["x"] * 2
+    for view in views.values():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            fresh = {k: v.detach().requires_grad_(True) for k, v in leaves.items()}
+            _apply(view(fresh), "silu")                      # (leaves of no other graph)
+            with pytest.raises(RuntimeError, match="eager graph"):
+                _apply(view({**fresh, "x": leaves["x"], "w_up": leaves["w_up"]}), "silu")
+            with pytest.raises(RuntimeError, match="eager graph"):
+                _apply({**fresh, "x": between}, "silu")
+            _apply({**fresh, "x": between.detach()}, "silu")
+    del alive, fresh, between
+    gc.collect()                                             # (what the refused calls' tracebacks hold)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = _apply(views["cast"](leaves), "silu")
+        (got,) = torch.autograd.grad(y, [leaves["w_up"]], dy.bfloat16())
+    want = run({k: v.detach().bfloat16() for k, v in t.items()}, dy.bfloat16(), "silu")
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want["y"]) and torch.equal(got, want["d_w_up"].float())
