@@ -17,9 +17,9 @@
 //   K-strided tile, 32-bit: one 16-byte read serves four MFMA tiles whose columns are interleaved (n = 4 i + t).
 // Out-of-range rows read as zero through the buffer descriptor's bound; a contraction tail inside a row is masked per lane.
 //
-// Bound by the matrix cores and the LDS at large sizes (8192 x 4096 -> 11264 bf16, a pass: x W_gate | W_up 1260 us and 1200
-// TFLOP/s, h W_down^T 600 and 1260, dh 800 and 945 -- its epilogue reads a and b -- dx 1160 and 1300, the weight gradients 1940
-// and 1170; library products of this card 1490), by latency at small ones (8192 x 288 -> 256: 7 to 14 us a launch).
+// Bound by the matrix cores and the LDS at large sizes (8192 x 4096 -> 11264 bf16, a pass: x W_gate | W_up 1252 us and 1208
+// TFLOP/s, h W_down^T 593 and 1275, dh 800 and 945 -- its epilogue reads a and b -- dx 1168 and 1294, the weight gradients 1915
+// and 1184; library products of this card 1490), by latency at small ones (8192 x 288 -> 256: 7 to 15 us a launch).
 //
 // The accumulators are computed transposed (B as the first MFMA operand): a lane then holds consecutive columns of one row
 // of C and stores vectors.

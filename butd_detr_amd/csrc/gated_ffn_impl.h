@@ -10,13 +10,13 @@
 namespace ffn {
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------
-// Up to 16 rows, and up to 64 with small weights: the product reads every weight once and little else, so it is a stream of weights with 16 rows (a matrix
-// instruction's width) per accumulator tile.  A workgroup owns 16 output columns; its waves share out the contraction in
-// 128-byte pieces (whole lines of the weights' rows), load straight into fragments -- nothing is reused between waves, LDS
-// would only add a trip -- and join their sums in LDS.  Bound by the weights' stream: 1 row of 4096 -> 11264 bf16 33.5 + 16.7
-// us, 5.5 TB/s; 13 rows of 2048 -> 5632 fp16 14.4 + 11 us, of which 3 us are a launch's and a quarter the rows themselves, read
-// again for every 16 columns.  16 waves a workgroup, where there are fewer workgroups than CUs, change nothing for large
-// weights and cost up to a quarter for small ones.
+// Up to 16 rows, and up to 64 with small weights: the product reads every weight once and little else, so it is a stream of
+// weights with 16 rows (a matrix instruction's width) per accumulator tile.  A workgroup owns 16 output columns; its waves
+// share out the contraction in 128-byte pieces (whole lines of the weights' rows), load straight into fragments -- nothing is
+// reused between waves, LDS would only add a trip -- and join their sums in LDS.  Bound by the weights' stream: 1 row of 4096 ->
+// 11264 bf16 37.7 + 19.2 us, 4.9 TB/s; 13 rows of 2048 -> 5632 fp16 15.1 + 11.1 us, of which 3 us are a launch's and a quarter
+// the rows themselves, read again for every 16 columns.  16 waves a workgroup, where there are fewer workgroups than CUs, change
+// nothing for large weights and cost up to a quarter for small ones.
 template <typename T, bool AL> __device__ inline u32x4 load_unit(const T *p, int left) {
   u32x4 v;
   if constexpr (AL) {
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const FewRows P) {
 }
 
 // ---- rows that direct loads cannot take -----------------------------------------------------------------------------------
-// One pass over the operand, in the launch before the product (x and the three weights of 1003 x 777 -> 2051 fp16: 7 us).
+// One pass over the operand, in the launch before the product (x and the three weights of 1003 x 777 -> 2051 fp16: 6 us).
 struct Copy {
   const void *src;
   void *dst;
@@ -157,7 +157,7 @@ template <typename T> __global__ __launch_bounds__(256) void copy_rows_kernel(co
 }
 
 // ---- slabs of a split contraction -----------------------------------------------------------------------------------------
-// Memory bound: every slab once (2 slabs of 2048 x 4096 and a bf16 result, 84 MB: 13.6 us).  Atomics into one slab would
+// Memory bound: every slab once (2 slabs of 2048 x 4096 and a bf16 result, 84 MB: 13.9 us).  Atomics into one slab would
 // change the order of the sums from run to run.
 struct Fold {
   const float *slab;
@@ -210,7 +210,8 @@ template <typename T> __global__ __launch_bounds__(256) void fold_kernel(const F
 
 // ---- bias gradients: sums over chunks of rows, folded like slabs -------------------------------------------------------------
 // Of dy itself, and of the column sums over each wave's rows that the product before took of da and db in 32 bits (from the
-// rounded da and db the sums' error is 1.57 times that of one rounding at the end, 8192 rows).
+// rounded da and db the sums' error is 1.57 times that of one rounding at the end, 8192 rows).  2048 x 288 -> 2048 fp32: 4.7 us,
+// a launch's.
 struct ColumnSum {
   const void *src;
   long rows, ld;               // ld in elements

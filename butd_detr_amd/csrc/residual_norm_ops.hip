@@ -3,9 +3,9 @@
 // Memory bound: forward reads x and residual and writes stream and normed, backward reads x, residual and the two arriving
 // gradients and writes two.  A row's values stay in registers from the load to the last use (both norms' statistics are
 // sums over registers, the deviations taken around the mean, not as a difference of squares), so each tensor is touched
-// once.  Measured (16384 rows of 4096, bf16 on a 32-bit stream, RMSNorm on both sides, a gate per channel): forward 148 us,
-// backward 237 us, sums of the parameters' gradients 4.4 us -- 5.2, 5.1 TB/s, the rate of a large copy; 8192 rows of 8192 bf16
-// forward 98 us.  2048 rows of 288 fp32, the layers' own: 5.2, 9.3 and 3.4 us, launches more than bytes.
+// once.  Measured (16384 rows of 4096, bf16 on a 32-bit stream, RMSNorm on both sides, a gate per channel): forward 146 us,
+// backward 239 us, sums of the parameters' gradients 4.7 us -- 5.5, 5.1 TB/s (a large copy: 5.15); 8192 rows of 8192 bf16 forward
+// 98 us, 5.5 TB/s.  2048 rows of 288 fp32, the layers' own: 5.6, 9.6 and 4.1 us, launches more than bytes.
 // Rows of up to 512 elements belong to ONE wave and are reduced inside it; wider rows to a workgroup.  Rows of any
 // width and address, 16 bytes a lane.
 #include <hip/hip_runtime.h>

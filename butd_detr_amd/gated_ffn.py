@@ -4,10 +4,12 @@
 
 -- the gated variant of the FFN of the encoder / decoder layers (models/encoder_decoder_layers.py:110-122,315-323 build
 Linear-ReLU-Linear), for fp32, bf16 and fp16 tensors.  Forward is two launches (both projections, the activation and the
-product are one kernel), backward three to seven.  Up to 16 rows -- a token each of a few sequences; up to 64 where the
-weights are small -- take kernels that do nothing but stream the weights.  The precision is the tensors' own (``fused_attention.set_compute_dtype`` does not apply):
-16-bit operands, everything between two products in 32 bits.  Checks, allocation and the autograd node are C++
-(binding/blocks_aten.cpp): a small layer is bound by the host.
+product are one kernel), with copies of odd rows and a split contraction's fold four; backward up to six.  Up to 16 rows -- a
+token each of a few sequences; up to 64 where the weights are small -- take kernels that do nothing but stream the weights.
+The precision is the tensors' own (``fused_attention.set_compute_dtype`` does not apply): 16-bit tensors are multiplied as they
+are and accumulated in 32 bits, with biases, activation and its derivative; h and the gradients of its two factors are operands
+of the next product and rounded to the tensors' type for it (fp16: an h beyond 65504 is infinite, as behind an fp16 linear
+layer).  Checks, allocation and the autograd node are C++ (binding/blocks_aten.cpp): a small layer is bound by the host.
 """
 from torch import nn
 
