@@ -153,14 +153,17 @@ def gated_ffn(ffn, x):
     return ffn.down(act(ffn.gate(x)) * ffn.up(x))
 
 
-def _wide_norm(norm, v):
-    """norm(v) for v in 32 bits or more and parameters of any type."""
-    weight, bias = (None if p is None else p.to(v.dtype) for p in (getattr(norm, "weight", None), getattr(norm, "bias", None)))
+def _wide_norm(norm, v, dtype):
+    """norm(v) for v in 32 bits or more: LayerNorm and RMSNorm with parameters of any type, other modules on v's ``dtype`` form."""
+    if not isinstance(norm, (nn.LayerNorm, nn.RMSNorm)):
+        return norm(v.to(dtype)).to(v.dtype)
+    params = [getattr(norm, "weight", None), getattr(norm, "bias", None)]
+    if all(p is None or p.dtype == v.dtype for p in params):
+        return norm(v)
+    weight, bias = (None if p is None else p.to(v.dtype) for p in params)
     if isinstance(norm, nn.LayerNorm):
         return F.layer_norm(v, norm.normalized_shape, weight, bias, norm.eps)
-    if isinstance(norm, nn.RMSNorm):
-        return F.rms_norm(v, norm.normalized_shape, weight, norm.eps)
-    return norm(v)
+    return F.rms_norm(v, norm.normalized_shape, weight, norm.eps)
 
 
 def residual_norm(x, residual=None, *, post_norm=None, gate=None, residual_scale=1.0, pre_norm=None):
@@ -175,12 +178,12 @@ def residual_norm(x, residual=None, *, post_norm=None, gate=None, residual_scale
     wide = torch.promote_types(torch.promote_types(x.dtype, out), torch.float32)
     stream = x.to(wide)
     if post_norm is not None:
-        stream = _wide_norm(post_norm, stream)
+        stream = _wide_norm(post_norm, stream, x.dtype)
     if gate is not None:
         stream = stream * (gate[:, None, :] if x.dim() == 3 and gate.dim() == 2 else gate).to(wide)
     if residual is not None:
         stream = residual_scale * residual.to(wide) + stream
-    normed = None if pre_norm is None else _wide_norm(pre_norm, stream).to(x.dtype)
+    normed = None if pre_norm is None else _wide_norm(pre_norm, stream, out).to(x.dtype)
     return x if residual is None and gate is None and post_norm is None else stream.to(out), normed
 
 

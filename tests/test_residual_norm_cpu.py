@@ -160,3 +160,30 @@ def test_a_block_begins_a_stack_of_16_bit_blocks_on_a_32_bit_stream():
         ab.set_backend(prev)
     assert stream.dtype == torch.float32 and normed.dtype == torch.bfloat16
     assert torch.equal(stream, by_hand[0]) and torch.equal(normed, by_hand[1])
+
+
+def test_torch_backend_calls_other_modules_on_the_tensors_own_type():
+    from butd_detr_amd import attention_blocks as ab
+
+    class Scale(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w = nn.Linear(8, 8, bias=False, dtype=torch.bfloat16)
+
+        def forward(self, v):
+            return self.w(v)                                 # (raises on another type)
+
+    torch.manual_seed(3)
+    m, hooked, calls = Scale(), nn.LayerNorm(8), []
+    hooked.register_forward_hook(lambda *a: calls.append(1))
+    x, r = torch.randn(2, 3, 8).bfloat16(), torch.randn(2, 3, 8).bfloat16()
+    prev = ab.get_backend()
+    try:
+        ab.set_backend("torch")
+        stream, normed = ab.residual_norm(x, r, post_norm=m, pre_norm=m)
+        assert stream.dtype == normed.dtype == torch.bfloat16
+        assert torch.equal(stream, (r.float() + m(x).float()).bfloat16()) and torch.equal(normed, m(stream))
+        ab.residual_norm(x.float(), r.float(), pre_norm=hooked)
+        assert calls == [1]
+    finally:
+        ab.set_backend(prev)
