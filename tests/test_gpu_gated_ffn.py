@@ -578,3 +578,17 @@ def test_capture_beside_a_living_eager_graph_is_refused_for_casts_and_views():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want["y"]) and torch.equal(got, want["d_w_up"].float())
+
+
+def test_recomputed_and_offloaded_activations():
+    """torch.utils.checkpoint and saved tensors kept on the host: the same gradients, bit for bit"""
+    from torch.utils.checkpoint import checkpoint
+    t, dy = inputs(130, 40, 56, torch.bfloat16)
+    want = run(t, dy, "silu")
+    leaves = {k: v.requires_grad_(True) for k, v in t.items()}
+    ys = [checkpoint(lambda *a: _apply(dict(zip(leaves, a)), "silu"), *leaves.values(), use_reentrant=False)]
+    with torch.autograd.graph.save_on_cpu():
+        ys.append(_apply(leaves, "silu"))
+    for y in ys:
+        for k, g in zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)):
+            assert torch.equal(g, want["d_" + k]), k
